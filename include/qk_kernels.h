@@ -406,6 +406,109 @@ int qkk_dn_step_seq(const float *conv, const float *gb, float *state, const floa
                     float *att, uint32_t d_state, uint32_t hK, uint32_t hV, uint32_t kdiv, float eps,
                     uint32_t n_pos, void *stream);
 
+/* ---- a paged cache of keys and values, and the attention over runs of rows ---------------------------
+ * No counterpart in the reference, whose caches are one contiguous stripe per slot and whose prompts go
+ * through one slot at a time (reference src/main.cpp:3953-4090): one pass over the rows of SEVERAL
+ * sequences (prompts packed behind each other, or a tree of drafted tokens per sequence), on a cache whose
+ * rows lie in pages, so that sequences can share what they have in common.
+ *
+ * qkk_kv_cache: keys and values of n_layer layers, k and v [n_layer][n_page][n_kv][page_rows][dh] of
+ * `type` (QKK_F32 or QKK_F16; a value written to an F16 cache is rounded to nearest).  Row r of sequence s
+ * lies in page table[s][r / page_rows] as its row r % page_rows.  dh 128 or 256.
+ *   table  [n_seq][seq_pages] page ids, -1 where there is none; page_rows a power of two, 16..65536.
+ *          NULL: a slot cache -- sequence s IS page s (seq_pages 1, n_seq <= n_page, any page_rows up to
+ *          2^24): the caches of qkk_attn_prep / qkk_attn_decode are such a cache with one layer.
+ *   ref    [n_page] sequences that hold a page (0: free); len [n_seq] rows a sequence holds.  Read and
+ *          written by qkk_kv_resize / qkk_kv_fork only (ref: NULL for a slot cache).
+ * A page id outside 0..n_page-1 is never followed: its rows are not written, and no row sees them.
+ *
+ * qkk_kv_runs: n_rows activation rows, cut into n_run runs of consecutive rows.  Run i is the rows
+ * start[i] .. start[i+1]-1 (ascending, start[n_run] <= n_rows; empty runs are allowed; rows in no run are
+ * left as they were), belongs to sequence seq[i], and its first row is cache row pos[i].  No run is longer
+ * than max_run (rows behind that are left as they were): it chooses the launch shape.  start, seq and pos
+ * are DEVICE arrays, so a captured graph follows them.  A run with seq or pos out of range is left out. */
+typedef struct qkk_kv_cache {
+    int32_t type;
+    uint32_t n_layer, n_page, n_kv, page_rows, dh, n_seq, seq_pages;
+    void *k, *v;
+    int32_t *table, *ref, *len;
+} qkk_kv_cache;
+typedef struct qkk_kv_runs {
+    uint32_t n_rows, n_run, max_run;
+    const int32_t *start, *seq, *pos;
+} qkk_kv_runs;
+
+/* qkk_attn_prep over the rows of runs, with rotation angles from up to 8 position axes (time, height and
+ * width of an image's or a video's rows).  Per head RMS norm with q_norm_w / k_norm_w; then pair j (dims j
+ * and j + n_rot/2) is turned by the angle rope[p][j], p = axis_pos[pair_axis[j]][row] -- so the pairs may
+ * be dealt out to the axes in sections or in turn (qkk_rope_axes).  Queries go to qhat [n_rows][hQ][dh],
+ * keys and values to the row's place in layer `layer` of the cache.
+ *   q        [n_rows][hQ][dh], or with gated != 0 [n_rows][hQ][2*dh] (per head the query, then the gate's
+ *            pre-activation, as qkk_attn_prep takes it);  kin, vin [n_rows][n_kv][dh]
+ *   rope     [rope_rows][n_rot/2][2] (qkk_rope_table); a position outside it is clamped
+ *   pair_axis [n_rot/2] bytes, axis_pos [n_axis][n_rows], on the device
+ * qkk_rope_axes fills a host array axis_host[n_rot/2]: sections_host[a] pairs for axis a (their sum
+ * n_rot/2), one axis after the other, or (in_turn) dealt out in turn while an axis has pairs left. */
+#define QKK_MAX_AXES 8u
+int qkk_rope_axes(uint8_t *axis_host, uint32_t n_rot, const uint32_t *sections_host, uint32_t n_axis,
+                  int in_turn);
+int qkk_attn_prep_axes(const qkk_kv_cache *C_host, uint32_t layer, const qkk_kv_runs *R_host, const float *q,
+                       const float *kin, const float *vin, const float *q_norm_w, const float *k_norm_w,
+                       const float *rope, uint32_t rope_rows, const uint8_t *pair_axis, uint32_t n_axis,
+                       const int32_t *axis_pos, float *qhat, uint32_t hQ, uint32_t n_rot, int gated, float eps,
+                       void *stream);
+
+/* Attention of the rows of runs over the cache (their own keys and values are in it already):
+ *   att[row][h] = softmax(qhat[row][h] . K / sqrt(dh)) V over the cache rows that the row sees, of KV head
+ *   h / (hQ/n_kv), times sigmoid(qfull[row][h][dh..]) where qfull [n_rows][hQ][2*dh] is given (NULL: no gate).
+ * qkk_attn_packed  row t of a run sees cache rows 0 .. pos + t: prompts, or parts of prompts behind what
+ *                  the cache holds, packed one after the other.
+ * qkk_attn_tree    row t of a run is node t of a tree of drafted tokens: it sees the cache rows below
+ *                  pos, its ancestors' rows and its own.  parent [n_rows]: the node's parent within its
+ *                  run (below t); anything else makes the node a root.  max_run <= QKK_TREE_MAX.  A tree
+ *                  of one node is the decode step.
+ * A row that sees nothing gives zeros.  What a row does not see never enters its result, whatever the
+ * cache holds there; what it sees and is not finite makes it NaN or infinite.
+ * The softmax's maximum and sum and all sums are fp32.  Results do not depend on what else runs, and are
+ * the same bits from call to call.
+ *   workspace: qkk_attn_runs_workspace_bytes(), 256-byte aligned, no initialisation needed; calls (and
+ *   graphs) that share one must not overlap in time. */
+#define QKK_TREE_MAX 256u
+size_t qkk_attn_runs_workspace_bytes(const qkk_kv_cache *C_host, const qkk_kv_runs *R_host, uint32_t hQ);
+int qkk_attn_packed(const qkk_kv_cache *C_host, uint32_t layer, const qkk_kv_runs *R_host, const float *qhat,
+                    const float *qfull, float *att, void *workspace, size_t workspace_bytes, uint32_t hQ,
+                    void *stream);
+int qkk_attn_tree(const qkk_kv_cache *C_host, uint32_t layer, const qkk_kv_runs *R_host, const int32_t *parent,
+                  const float *qhat, const float *qfull, float *att, void *workspace, size_t workspace_bytes,
+                  uint32_t hQ, void *stream);
+
+/* The books of the pages, kept on the device (every array below is a device array, every call can be
+ * captured), one call for all layers.
+ * qkk_kv_resize  len_new [n_seq]: the rows each sequence is to hold; -1 leaves it as it is, 0 frees it.
+ *                A shorter one gives back the pages behind its end (a page is free when no sequence holds
+ *                it).  A longer one takes the free pages with the lowest ids, sequences in ascending
+ *                order; pages freed by the same call may be taken.  If its part-filled last page is held
+ *                by another sequence too, it first gets a copy of its own of that page's rows -- so rows
+ *                from len on may always be written.  *status = 0; or the number of pages that are
+ *                missing: then no sequence grows (the shorter ones are cut); or -1: a length beyond
+ *                the sequence's pages, nothing is changed.  workspace: qkk_kv_workspace_bytes().
+ * qkk_kv_fork    for i < n: sequence dst[i], which must hold nothing, gets all rows of src[i] -- by sharing
+ *                its pages; in a slot cache by copying the rows.  *status = 0, or -1 if an id is out of
+ *                range, a dst holds rows or comes twice: then nothing is changed.  One src may come more than
+ *                once.  n <= n_seq.
+ * qkk_kv_compact for i < n: of the drafted rows behind cache row base[i] of sequence seq[i], row
+ *                base + path[i][j] is moved to base + j, j < n_path[i] (path [n][max_path], ascending):
+ *                the accepted path of a tree to the front.  A path that is not strictly ascending, or
+ *                leaves the sequence's pages, is left out (nothing of it is moved).  Touches no books; each
+ *                sequence once.  max_path <= QKK_TREE_MAX. */
+size_t qkk_kv_workspace_bytes(const qkk_kv_cache *C_host);
+int qkk_kv_resize(const qkk_kv_cache *C_host, const int32_t *len_new, int32_t *status, void *workspace,
+                  size_t workspace_bytes, void *stream);
+int qkk_kv_fork(const qkk_kv_cache *C_host, const int32_t *src, const int32_t *dst, uint32_t n, int32_t *status,
+                void *workspace, size_t workspace_bytes, void *stream);
+int qkk_kv_compact(const qkk_kv_cache *C_host, const int32_t *seq, const int32_t *base, const int32_t *path,
+                   const int32_t *n_path, uint32_t n, uint32_t max_path, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,6 +14,8 @@ from .capi import (  # noqa: F401
     rope_table, attn_prep, attn_workspace_bytes, attn_decode, dn_ab, dn_conv, dn_step, dn_ab_conv,
     moe_decode_static, moe_workspace_status, gemv_norm, head_argmax_norm, dn_step_fused, MOE_STATIC_MAX_SLOTS, MOE_STATIC_BYTES,
     set_option, get_option, option,
+    KvCache, KvRuns, rope_axes, attn_prep_axes, attn_runs_workspace_bytes, attn_packed, attn_tree, kv_workspace_bytes, kv_resize, kv_fork,
+    kv_compact,
 )
 from . import capi  # noqa: F401
 from . import synth  # noqa: F401

@@ -27,6 +27,15 @@ class _Layer(C.Structure):
                 ("up_shexp", C.c_void_p), ("down_shexp", C.c_void_p)]
 
 
+class _KvCache(C.Structure):
+    _fields_ = [("type", C.c_int32)] + [(n, C.c_uint32) for n in ("n_layer", "n_page", "n_kv", "page_rows", "dh", "n_seq", "seq_pages")] + \
+               [(n, C.c_void_p) for n in ("k", "v", "table", "ref", "len")]
+
+
+class _KvRuns(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("n_rows", "n_run", "max_run")] + [(n, C.c_void_p) for n in ("start", "seq", "pos")]
+
+
 def lib_path():
     return os.path.join(os.path.dirname(os.path.abspath(__file__)), "libqk.so")
 
@@ -85,6 +94,15 @@ def _signatures():
         "qkk_attn_prep_seq": (None, attn_prep),
         "qkk_attn_decode": (None, attn_decode),
         "qkk_attn_seq": (None, attn_decode),
+        "qkk_rope_axes": (None, [vp, u32, vp, u32, i32]),
+        "qkk_attn_prep_axes": (None, [vp, u32, vp] + [vp] * 6 + [u32, vp, u32, vp, vp, u32, u32, i32, f32, vp]),
+        "qkk_attn_runs_workspace_bytes": (sz, [vp, vp, u32]),
+        "qkk_attn_packed": (None, [vp, u32] + [vp] * 5 + [sz, u32, vp]),
+        "qkk_attn_tree": (None, [vp, u32] + [vp] * 6 + [sz, u32, vp]),
+        "qkk_kv_workspace_bytes": (sz, [vp]),
+        "qkk_kv_resize": (None, [vp] * 4 + [sz, vp]),
+        "qkk_kv_fork": (None, [vp] * 3 + [u32, vp, vp, sz, vp]),
+        "qkk_kv_compact": (None, [vp] * 5 + [u32, u32, vp]),
     }
 
 
@@ -535,3 +553,183 @@ def dn_step(conv, gb, state, norm_w, z, hK, hV, kdiv=0, d_state=128, eps=1e-6, a
     fn = lib().qkk_dn_step_seq if seq else lib().qkk_dn_step
     _check(fn(_ptr(conv), _ptr(gb), _ptr(state), _ptr(norm_w), _ptr(z), _ptr(att), d_state, hK, hV, kdiv, eps, n, _stream()))
     return att
+
+
+# ---- the paged cache and the attention over runs of rows ------------------------------------------
+
+def _want(who, device, **tensors):
+    """Each named (tensor, dtype, shape or None): on the device of the cache, contiguous, of that type and shape."""
+    for name, (t, dtype, shape) in tensors.items():
+        if t is None:
+            continue
+        if t.device != device or t.dtype != dtype or not t.is_contiguous() or (shape is not None and tuple(t.shape) != tuple(shape)):
+            raise ValueError(f"{who}: {name} must be a contiguous {dtype} tensor" + (f" of shape {tuple(shape)}" if shape is not None else "") +
+                             f" on {device}, not {t.dtype} {tuple(t.shape)} on {t.device}" + ("" if t.is_contiguous() else " (strided)"))
+
+
+def _here(who, device):
+    """The calls go to the current device's current stream: the cache has to be there."""
+    if device.type == "cuda":
+        import torch
+        if device.index != torch.cuda.current_device():
+            raise ValueError(f"{who}: the cache is on {device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+class KvCache:
+    """A cache of keys and values [n_layer][n_page][n_kv][page_rows][dh] (float32 or float16).  table int32 [n_seq][seq_pages]
+    names the pages of each sequence (-1: none), ref int32 [n_page] counts who holds a page, len int32 [n_seq] the rows
+    held (both for kv_resize / kv_fork only).  Without a table sequence s is page s."""
+
+    def __init__(self, k, v, table=None, ref=None, len=None, n_seq=None):
+        import torch
+        types = {torch.float32: F32, torch.float16: F16}
+        if k.dim() != 5 or k.dtype not in types:
+            raise ValueError("KvCache: k must be a float32 or float16 tensor [n_layer][n_page][n_kv][page_rows][dh]")
+        n_layer, n_page, n_kv, page_rows, dh = k.shape
+        if table is not None:
+            if table.dim() != 2 or (n_seq is not None and n_seq != table.shape[0]):
+                raise ValueError("KvCache: table must be [n_seq][seq_pages]")
+            n_seq, seq_pages = table.shape
+        else:
+            n_seq, seq_pages = n_page if n_seq is None else n_seq, 1
+        i32 = torch.int32
+        _want("KvCache", k.device, k=(k, k.dtype, None), v=(v, k.dtype, k.shape), table=(table, i32, None), ref=(ref, i32, (n_page,)),
+              len=(len, i32, (n_seq,)))
+        self.k, self.v, self.table, self.ref, self.len = k, v, table, ref, len
+        self.n_layer, self.n_page, self.n_kv, self.page_rows, self.dh = n_layer, n_page, n_kv, page_rows, dh
+        self.n_seq, self.seq_pages, self.device = n_seq, seq_pages, k.device
+        at = [0 if t is None else t.data_ptr() for t in (k, v, table, ref, len)]
+        self.c = _KvCache(types[k.dtype], n_layer, n_page, n_kv, page_rows, dh, n_seq, seq_pages, *at)
+        self.ref_c = C.byref(self.c)
+
+
+class KvRuns:
+    """n_rows activation rows cut into runs: run i is the rows start[i] .. start[i+1]-1, of sequence seq[i], its first row cache row
+    pos[i].  start int32 [n_run+1], seq and pos int32 [n_run], on the device (their values may change between calls).  max_run: no
+    run is longer (default n_rows)."""
+
+    def __init__(self, n_rows, start, seq, pos, max_run=None):
+        import torch
+        n_run = seq.numel()
+        i32 = torch.int32
+        _want("KvRuns", seq.device, seq=(seq, i32, (n_run,)), start=(start, i32, (n_run + 1,)), pos=(pos, i32, (n_run,)))
+        self.start, self.seq, self.pos, self.n_rows, self.n_run, self.device = start, seq, pos, n_rows, n_run, seq.device
+        self.max_run = n_rows if max_run is None else max_run
+        self.c = _KvRuns(n_rows, n_run, self.max_run, start.data_ptr(), seq.data_ptr(), pos.data_ptr())
+        self.ref_c = C.byref(self.c)
+
+
+def rope_axes(n_rot, sections, in_turn=False):
+    """uint8 numpy array [n_rot/2]: the axis of each rotated pair, sections[a] pairs for axis a, one axis after the other or
+    (in_turn) dealt out in turn."""
+    import numpy as np
+    out = np.zeros(max(n_rot // 2, 1), dtype=np.uint8)
+    sec = (C.c_uint32 * max(len(sections), 1))(*sections)
+    _check(lib().qkk_rope_axes(out.ctypes.data_as(C.c_void_p), n_rot, sec, len(sections), int(in_turn)))
+    return out
+
+
+def attn_prep_axes(cache, layer, runs, q, kin, vin, q_norm_w, k_norm_w, rope, pair_axis, axis_pos, eps=1e-6, qhat=None):
+    """Head norm, rotation with several position axes, cache write for the rows of runs.  q [rows][hQ][dh], or [rows][hQ][2*dh] with
+    the output gate behind each head's query; kin / vin [rows][n_kv][dh]; rope [rope_rows][n_rot/2][2]; pair_axis uint8
+    [n_rot/2]; axis_pos int32 [n_axis][rows].  Returns qhat [rows][hQ][dh]."""
+    import torch
+    f, rows, dh = torch.float32, runs.n_rows, cache.dh
+    hQ = q.shape[1] if q.dim() == 3 else 0
+    if q.dim() != 3 or q.shape[2] not in (dh, 2 * dh) or rope.dim() != 3 or rope.shape[2] != 2 or axis_pos.dim() != 2:
+        raise ValueError("attn_prep_axes: q must be [rows][hQ][dh or 2*dh], rope [rope_rows][n_rot/2][2], axis_pos [n_axis][rows]")
+    _here("attn_prep_axes", cache.device)
+    if qhat is None:
+        qhat = torch.empty((rows, hQ, dh), dtype=f, device=q.device)
+    _want("attn_prep_axes", cache.device, start=(runs.start, torch.int32, None), q=(q, f, (rows, hQ, q.shape[2])), kin=(kin, f, (rows, cache.n_kv, dh)),
+          vin=(vin, f, (rows, cache.n_kv, dh)), q_norm_w=(q_norm_w, f, (dh,)), k_norm_w=(k_norm_w, f, (dh,)), rope=(rope, f, None),
+          pair_axis=(pair_axis, torch.uint8, (rope.shape[1],)), axis_pos=(axis_pos, torch.int32, (axis_pos.shape[0], rows)), qhat=(qhat, f, (rows, hQ, dh)))
+    _check(lib().qkk_attn_prep_axes(cache.ref_c, layer, runs.ref_c, _ptr(q), _ptr(kin), _ptr(vin), _ptr(q_norm_w), _ptr(k_norm_w), _ptr(rope),
+                                    rope.shape[0], _ptr(pair_axis), axis_pos.shape[0], _ptr(axis_pos), _ptr(qhat), hQ, 2 * rope.shape[1],
+                                    int(q.shape[2] != dh), eps, _stream()))
+    return qhat
+
+
+def attn_runs_workspace_bytes(cache, runs, hQ):
+    return lib().qkk_attn_runs_workspace_bytes(cache.ref_c, runs.ref_c, hQ)
+
+
+def _attn_runs(who, cache, layer, runs, parent, qhat, workspace, qfull, att):
+    import torch
+    f, rows = torch.float32, runs.n_rows
+    if qhat.dim() != 3:
+        raise ValueError(f"{who}: qhat must be [rows][hQ][dh]")
+    hQ, dh = qhat.shape[1], cache.dh
+    _here(who, cache.device)
+    if att is None:
+        att = torch.empty_like(qhat)
+    _want(who, cache.device, start=(runs.start, torch.int32, None), qhat=(qhat, f, (rows, hQ, dh)), att=(att, f, (rows, hQ, dh)),
+          qfull=(qfull, f, (rows, hQ, 2 * dh)), parent=(parent, torch.int32, (rows,)), workspace=(workspace, workspace.dtype, None))
+    nbytes = workspace.numel() * workspace.element_size()
+    if parent is None:
+        _check(lib().qkk_attn_packed(cache.ref_c, layer, runs.ref_c, _ptr(qhat), _ptr(qfull), _ptr(att), _ptr(workspace), nbytes, hQ, _stream()))
+    else:
+        _check(lib().qkk_attn_tree(cache.ref_c, layer, runs.ref_c, _ptr(parent), _ptr(qhat), _ptr(qfull), _ptr(att), _ptr(workspace), nbytes, hQ,
+                                   _stream()))
+    return att
+
+
+def attn_packed(cache, layer, runs, qhat, workspace, qfull=None, att=None):
+    """Attention of packed prompts: row t of a run sees cache rows 0 .. pos + t of its sequence.  qhat [rows][hQ][dh]; qfull
+    [rows][hQ][2*dh]: the output gate's pre-activations in the second halves (None: no gate).  Returns att [rows][hQ][dh]."""
+    return _attn_runs("attn_packed", cache, layer, runs, None, qhat, workspace, qfull, att)
+
+
+def attn_tree(cache, layer, runs, parent, qhat, workspace, qfull=None, att=None):
+    """Attention of trees of drafted tokens: row t of a run sees the cache rows below pos, its ancestors' rows and its own.
+    parent int32 [rows]: the parent's index within its run, -1 for a root.  Returns att [rows][hQ][dh]."""
+    if parent is None:
+        raise ValueError("attn_tree: parent is missing")
+    return _attn_runs("attn_tree", cache, layer, runs, parent, qhat, workspace, qfull, att)
+
+
+def kv_workspace_bytes(cache):
+    return lib().qkk_kv_workspace_bytes(cache.ref_c)
+
+
+def _status(who, cache, status, workspace):
+    import torch
+    _here(who, cache.device)
+    if status is None:
+        status = torch.empty(1, dtype=torch.int32, device=cache.device)
+    _want(who, cache.device, status=(status, torch.int32, (1,)), workspace=(workspace, workspace.dtype, None))
+    return status
+
+
+def kv_resize(cache, len_new, workspace, status=None):
+    """Sets the rows each sequence holds (int32 [n_seq]; -1: as it is, 0: freed); pages are freed and taken, a shared part-filled page is
+    copied before its sequence grows.  Returns the device status word: 0, the number of missing pages (nothing grew), or -1."""
+    import torch
+    status = _status("kv_resize", cache, status, workspace)
+    _want("kv_resize", cache.device, len_new=(len_new, torch.int32, (cache.n_seq,)))
+    _check(lib().qkk_kv_resize(cache.ref_c, _ptr(len_new), _ptr(status), _ptr(workspace), workspace.numel() * workspace.element_size(), _stream()))
+    return status
+
+
+def kv_fork(cache, src, dst, workspace, status=None):
+    """Sequences dst (empty) get the rows of src, sharing their pages (a slot cache: copies of the rows).  Returns the device status
+    word: 0, or -1 where nothing was changed."""
+    import torch
+    status = _status("kv_fork", cache, status, workspace)
+    n = src.numel()
+    _want("kv_fork", cache.device, src=(src, torch.int32, (n,)), dst=(dst, torch.int32, (n,)))
+    _check(lib().qkk_kv_fork(cache.ref_c, _ptr(src), _ptr(dst), n, _ptr(status), _ptr(workspace), workspace.numel() * workspace.element_size(),
+                             _stream()))
+    return status
+
+
+def kv_compact(cache, seq, base, path, n_path):
+    """Moves the accepted rows base + path[i][j] of sequence seq[i] to base + j, j < n_path[i], in all layers; path int32 [n][max_path],
+    ascending per path."""
+    import torch
+    i32, n = torch.int32, seq.numel()
+    if path.dim() != 2:
+        raise ValueError("kv_compact: path must be [n][max_path]")
+    _here("kv_compact", cache.device)
+    _want("kv_compact", cache.device, seq=(seq, i32, (n,)), base=(base, i32, (n,)), path=(path, i32, (n, path.shape[1])), n_path=(n_path, i32, (n,)))
+    _check(lib().qkk_kv_compact(cache.ref_c, _ptr(seq), _ptr(base), _ptr(path), _ptr(n_path), n, path.shape[1], _stream()))

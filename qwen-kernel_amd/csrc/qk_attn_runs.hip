@@ -1,0 +1,146 @@
+// qk_attn_runs.hip -- attention of runs of rows over the paged cache (qkk_attn_packed, qkk_attn_tree).
+//   att = softmax(q . K / sqrt(dh)) V * sigmoid(gate) over the cache rows a row sees: 0 .. pos + t of its sequence, or
+//   for a tree the rows below pos, the node's ancestors and itself.
+// The one-sequence forms on a slot's own cache are in qk_attn.hip.
+#include "qk_kv.h"
+
+#include <algorithm>
+
+namespace qk {
+
+constexpr uint32_t AR_TILE = 64;  // cache rows scored per pass
+constexpr float AR_FLOOR = -3.0e38f;
+
+// grid (rows, hQ), 256 threads: one row's head, tile after tile of the cache with the running maximum and sum.
+template <int DH, typename T, bool TREE>
+__global__ __launch_bounds__(256) void attn_runs_plain_kernel(KvView c, RunsView R, const int32_t* __restrict__ parent,
+                                                              const float* __restrict__ q, const float* __restrict__ qfull,
+                                                              float* __restrict__ att, uint32_t hQ)
+{
+    __shared__ float s_q[DH], s_p[AR_TILE], s_acc[256], s_m, s_l, s_corr;
+    __shared__ uint32_t s_kin[QKK_TREE_MAX / 32];
+    const uint32_t row = blockIdx.x, h = blockIdx.y, t = threadIdx.x, lane = t & 63u, wave = t >> 6;
+    const uint32_t ri = wave_last_le(R.n_run, row, [&](uint32_t i) { return (int64_t)R.start[i]; });
+    if (ri >= R.n_run) return; // the whole workgroup
+    const Run u = run_at(c, R, ri);
+    if (!u.ok || row - u.r0 >= u.n) return; // the whole workgroup
+    const uint32_t node = row - u.r0, kv = h / (hQ / c.n_kv);
+    for (uint32_t d = t; d < DH; d += 256) s_q[d] = q[((size_t)row * hQ + h) * DH + d];
+    if (t < QKK_TREE_MAX / 32) s_kin[t] = 0;
+    if (t == 0) { s_m = AR_FLOOR; s_l = 0.f; }
+    __syncthreads();
+    if (TREE && t == 0)
+        for (int32_t a = (int32_t)node;;) {
+            s_kin[a >> 5] |= 1u << (a & 31);
+            const int32_t up = parent[u.r0 + a];
+            if (up < 0 || up >= a) break;
+            a = up;
+        }
+    __syncthreads();
+    const float qs = 1.f / sqrtf((float)DH);
+    const T* K = (const T*)c.k;
+    const T* V = (const T*)c.v;
+    constexpr uint32_t PARTS = 256 / DH; // threads that share a dim
+    float acc = 0.f;
+    const uint32_t end = min(u.pos + node + 1, c.cap);
+    for (uint32_t p0 = 0; p0 < end; p0 += AR_TILE) {
+        // scores: 4 lanes per key
+        const uint32_t key = p0 + (t >> 2);
+        float s = 0.f;
+        bool sees = key < end && (!TREE || key < u.pos || ((s_kin[(key - u.pos) >> 5] >> ((key - u.pos) & 31)) & 1u));
+        const uint32_t page = sees ? kv_page(c, u.seq, key) : KV_NO_PAGE;
+        sees = page != KV_NO_PAGE;
+        if (sees) {
+            const T* row_k = K + kv_row(c, page, kv, key, DH);
+            for (uint32_t d = t & 3u; d < DH; d += 4) s += s_q[d] * (float)row_k[d];
+        }
+        s = group_sum<4>(s);
+        if ((t & 3u) == 0) s_p[t >> 2] = sees ? s * qs : -INFINITY;
+        __syncthreads();
+        if (wave == 0) {
+            const float v = s_p[lane];
+            const float m = fmaxf(s_m, wave_max(v));
+            const float e = v == -INFINITY ? 0.f : expf(v - m), sum = wave_sum(e);
+            s_p[lane] = v == -INFINITY ? -1.f : e; // negative: not seen
+            if (lane == 0) {
+                s_corr = expf(s_m - m);
+                s_l = s_l * s_corr + sum;
+                s_m = m;
+            }
+        }
+        __syncthreads();
+        acc *= s_corr;
+        const uint32_t d = t % DH;
+        for (uint32_t i = t / DH; i < AR_TILE && p0 + i < end; i += PARTS)
+            if (s_p[i] >= 0.f || s_p[i] != s_p[i]) acc += s_p[i] * (float)V[kv_row(c, kv_page(c, u.seq, p0 + i), kv, p0 + i, DH) + d];
+        __syncthreads(); // the next tile overwrites the scores
+    }
+    s_acc[t] = acc;
+    __syncthreads();
+    if (t < DH) {
+        float o = 0.f;
+        for (uint32_t i = 0; i < PARTS; i++) o += s_acc[t + i * DH];
+        o = s_l == 0.f ? 0.f : o / s_l;
+        if (qfull) o *= 1.f / (1.f + expf(-qfull[((size_t)row * hQ + h) * 2 * DH + DH + t]));
+        att[((size_t)row * hQ + h) * DH + t] = o;
+    }
+}
+
+static int attn_runs(const char* who, const qkk_kv_cache* C, uint32_t layer, const qkk_kv_runs* R, const int32_t* parent, bool tree,
+                     const float* qhat, const float* qfull, float* att, void* workspace, size_t workspace_bytes, uint32_t hQ, void* stream)
+{
+    KvView c;
+    RunsView runs;
+    if (int rc = kv_view(who, C, layer, &c)) return rc;
+    if (int rc = runs_view(who, R, &runs)) return rc;
+    if (!qhat || !att || !workspace || (tree && !parent)) return fail(QKK_EINVAL, "%s: null pointer", who);
+    if (hQ < c.n_kv || hQ % c.n_kv || hQ > 4096)
+        return fail(QKK_ESHAPE, "%s: %u query heads on %u KV heads not supported (a multiple, at most 4096)", who, hQ, c.n_kv);
+    if (tree && runs.max_run > QKK_TREE_MAX) return fail(QKK_ESHAPE, "%s: trees of up to %u nodes (at most %u)", who, runs.max_run, QKK_TREE_MAX);
+    if (!aligned16(qhat) || !aligned16(att) || !aligned16(qfull) || (reinterpret_cast<uintptr_t>(workspace) & 255u))
+        return fail(QKK_EINVAL, "%s: qhat, qfull and att must be 16-byte, workspace 256-byte aligned", who);
+    const size_t want = qkk_attn_runs_workspace_bytes(C, R, hQ);
+    if (workspace_bytes < want) return fail(QKK_EWORKSPACE, "%s: workspace %zu < %zu bytes", who, workspace_bytes, want);
+    if (int rc = require_device()) return rc;
+    if (!runs.n_rows || !runs.n_run) return QKK_OK;
+    const dim3 grid(runs.n_rows, hQ), block(256);
+#define QK_RUNS(DH, T, TREE)                                                                                                             \
+    hipLaunchKernelGGL((attn_runs_plain_kernel<DH, T, TREE>), grid, block, 0, as_stream(stream), c, runs, parent, qhat, qfull, att, hQ)
+#define QK_RUNS2(DH, T) do { if (tree) QK_RUNS(DH, T, true); else QK_RUNS(DH, T, false); } while (0)
+    if (C->dh == 256) {
+        if (C->type == QKK_F32) QK_RUNS2(256, float);
+        else QK_RUNS2(256, _Float16);
+    } else {
+        if (C->type == QKK_F32) QK_RUNS2(128, float);
+        else QK_RUNS2(128, _Float16);
+    }
+#undef QK_RUNS2
+#undef QK_RUNS
+    return check_launch(who);
+}
+
+} // namespace qk
+
+using namespace qk;
+
+extern "C" {
+
+size_t qkk_attn_runs_workspace_bytes(const qkk_kv_cache* C, const qkk_kv_runs* R, uint32_t hQ)
+{
+    if (!C || !R || !hQ) return 0;
+    return 256;
+}
+
+int qkk_attn_packed(const qkk_kv_cache* C, uint32_t layer, const qkk_kv_runs* R, const float* qhat, const float* qfull, float* att,
+                    void* workspace, size_t workspace_bytes, uint32_t hQ, void* stream)
+{
+    return attn_runs("qkk_attn_packed", C, layer, R, nullptr, false, qhat, qfull, att, workspace, workspace_bytes, hQ, stream);
+}
+
+int qkk_attn_tree(const qkk_kv_cache* C, uint32_t layer, const qkk_kv_runs* R, const int32_t* parent, const float* qhat, const float* qfull,
+                  float* att, void* workspace, size_t workspace_bytes, uint32_t hQ, void* stream)
+{
+    return attn_runs("qkk_attn_tree", C, layer, R, parent, true, qhat, qfull, att, workspace, workspace_bytes, hQ, stream);
+}
+
+} // extern "C"
