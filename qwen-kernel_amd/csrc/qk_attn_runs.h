@@ -1,0 +1,144 @@
+// qk_attn_runs.h -- what the kernels of qkk_attn_packed / qkk_attn_tree share (qk_attn_runs.hip, qk_attn_few.hip,
+// qk_attn_tile.hip).
+//
+// Both kernels compute, per KV head, the TRANSPOSED products on the matrix cores (v_mfma_f32_16x16x32, A 16 x 32, B
+// 32 x 16, D 16 x 16):
+//   S^T[key][row] = K[key][:] . Q[row][:]       A = 16 keys, B = 16 query rows
+//   O^T[dim][row] = V^T[dim][:] . P^T[:][row]   A = 16 dims, B = 16 query rows
+// so that a lane's outputs all belong to ONE query row (lane % 16): the running maximum, the sum and the rescaling are
+// lane-local up to one exchange between the four lane groups, and the weights P leave the first product in the
+// registers in which the second one wants them.  With g = lane / 16 a lane holds, after two S^T blocks of 16 keys, the
+// keys 4g .. 4g+3 and 16+4g .. 16+4g+3 of a step of 32; the second product contracts its 32 keys in exactly
+// that order (contraction order is free as long as A and B agree).
+//
+// The query rows of a run that share a KV head (positions x heads of the group) are numbered f = position * G + head, so
+// any group size fills the 16 columns.
+//
+// Two halves hold an fp32 value to 2^-22 inside a half's range, three bf16 pieces hold it exactly in fp32's own range:
+// products of split operands give fp32 results on the matrix cores (the kernels say which they use and why).
+#pragma once
+#include "qk_kv.h"
+#include "qk_mfma.h"
+
+namespace qk {
+
+constexpr float AR_FLOOR = -3.0e38f;
+constexpr float AR_LOG2E = 1.44269504088896341f;
+
+// One call.  Keys are cut into ranges of `chunk` rows (a multiple of 128), n_split of them cover the cache; with n_split 1 the
+// kernels write att, else each range's (maximum, sum, weighted sum) go to the workspace and attn_join_kernel folds them.
+struct RunsCall {
+    KvView c;
+    RunsView R;
+    const int32_t* parent;
+    const float *q, *qfull;
+    float *att, *acc, *ml; // acc [row][head][n_split][dh], ml [row][head][n_split][2] (log2 domain)
+    uint32_t hQ, G, n_split, chunk;
+};
+
+__device__ __forceinline__ float xor_lanes_max(float v) // over the four lane groups: lanes with the same lane % 16
+{
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float xor_lanes_sum(float v)
+{
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float4v mfma16x32(bf16x8 a, bf16x8 b, float4v c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ uint32_t f2u(float x) { return __builtin_bit_cast(uint32_t, x); }
+__device__ __forceinline__ float u2f(uint32_t x) { return __builtin_bit_cast(float, x); }
+
+// Eight floats as three bf16 vectors whose sum they are, exactly (8 bits each, truncated): infinities and NaN become NaN.
+struct Bf3 {
+    bf16x8 p[3];
+};
+__device__ __forceinline__ Bf3 split3(const float* x)
+{
+    u32x4 o[3];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+        for (int j = 0; j < 3; j++) {
+            o[j][i] = __builtin_amdgcn_perm(f2u(b), f2u(a), 0x07060302u); // upper halves of a, b
+            if (j < 2) {
+                a -= u2f(f2u(a) & 0xFFFF0000u);
+                b -= u2f(f2u(b) & 0xFFFF0000u);
+            }
+        }
+    }
+    Bf3 r;
+#pragma unroll
+    for (int j = 0; j < 3; j++) r.p[j] = __builtin_bit_cast(bf16x8, o[j]);
+    return r;
+}
+
+// Eight floats as hi + lo halves, both rounded to nearest: exact to 2^-22 of x while x is inside a half's normal range.
+struct Half2 {
+    half8 hi, lo;
+};
+__device__ __forceinline__ uint32_t pack_half(float a, float b) { return __builtin_bit_cast(uint32_t, half2v{(_Float16)a, (_Float16)b}); }
+__device__ __forceinline__ Half2 split2(const float* x)
+{
+    u32x4 h, l;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t top = pack_half(x[2 * i], x[2 * i + 1]);
+        const half2v hv = __builtin_bit_cast(half2v, top);
+        h[i] = top;
+        l[i] = pack_half(x[2 * i] - (float)hv[0], x[2 * i + 1] - (float)hv[1]);
+    }
+    return Half2{__builtin_bit_cast(half8, h), __builtin_bit_cast(half8, l)};
+}
+
+// The power of two that brings a maximum of magnitudes into [1, 2): its exponent, limited to what the reciprocal can hold.
+__device__ __forceinline__ int top_exponent(float m)
+{
+    return min(max((int)(f2u(m) >> 23) - 127, -126), 126);
+}
+__device__ __forceinline__ float pow2i(int e) { return u2f((uint32_t)(e + 127) << 23); }
+
+// Ancestors of the nodes node0 .. node0 + n - 1 of a run as bits, kin[n][QKK_TREE_MAX / 32] in LDS; s_up: the run's parents
+// (QKK_TREE_MAX entries).  The whole workgroup calls it (two barriers).
+__device__ __forceinline__ void tree_bits(const int32_t* __restrict__ parent, const Run& u, uint32_t node0, uint32_t n, int32_t* s_up,
+                                          uint32_t (*kin)[QKK_TREE_MAX / 32])
+{
+    for (uint32_t i = threadIdx.x; i < u.n; i += blockDim.x) s_up[i] = parent[u.r0 + i];
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
+        uint32_t w[QKK_TREE_MAX / 32] = {};
+#pragma unroll
+        for (uint32_t b = 0; b < QKK_TREE_MAX / 32; b++) w[b] = 0;
+        int32_t a = (int32_t)(node0 + i);
+        while (true) { // ends: a parent lies below its node
+#pragma unroll
+            for (uint32_t b = 0; b < QKK_TREE_MAX / 32; b++) w[b] |= (uint32_t)(a >> 5) == b ? 1u << (a & 31) : 0u;
+            const int32_t up = s_up[a];
+            if (up < 0 || up >= a) break;
+            a = up;
+        }
+#pragma unroll
+        for (uint32_t b = 0; b < QKK_TREE_MAX / 32; b++) kin[i][b] = w[b];
+    }
+    __syncthreads();
+}
+
+// rows x heads of a run that fit the kernel for few rows: one block of 16, for dh 128 two (at dh 256 a second block's accumulators
+// do not fit the registers)
+constexpr uint32_t few_rows(uint32_t dh) { return dh == 128 ? 32 : 16; }
+
+void launch_attn_few(const RunsCall& call, int type, uint32_t dh, bool tree, hipStream_t st);
+
+} // namespace qk

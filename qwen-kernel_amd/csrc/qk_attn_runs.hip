@@ -2,14 +2,13 @@
 //   att = softmax(q . K / sqrt(dh)) V * sigmoid(gate) over the cache rows a row sees: 0 .. pos + t of its sequence, or
 //   for a tree the rows below pos, the node's ancestors and itself.
 // The one-sequence forms on a slot's own cache are in qk_attn.hip.
-#include "qk_kv.h"
+#include "qk_attn_runs.h"
 
 #include <algorithm>
 
 namespace qk {
 
 constexpr uint32_t AR_TILE = 64;  // cache rows scored per pass
-constexpr float AR_FLOOR = -3.0e38f;
 
 // grid (rows, hQ), 256 threads: one row's head, tile after tile of the cache with the running maximum and sum.
 template <int DH, typename T, bool TREE>
@@ -86,6 +85,77 @@ __global__ __launch_bounds__(256) void attn_runs_plain_kernel(KvView c, RunsView
     }
 }
 
+// One wave per (row, head): folds the ranges in range order and applies the gate.  Ranges behind the row's own position hold
+// nothing for it.
+template <int DH>
+__global__ __launch_bounds__(256) void attn_join_kernel(RunsCall a)
+{
+    constexpr uint32_t PER = DH / 64;
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint64_t job = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const uint32_t row = (uint32_t)(job / a.hQ), h = (uint32_t)(job % a.hQ);
+    if (row >= a.R.n_rows) return; // the whole wave
+    const uint32_t ri = wave_last_le(a.R.n_run, row, [&](uint32_t i) { return (int64_t)a.R.start[i]; });
+    if (ri >= a.R.n_run) return;
+    const Run u = run_at(a.c, a.R, ri);
+    if (!u.ok || row - u.r0 >= u.n) return;
+    const uint32_t n = (min(u.pos + (row - u.r0) + 1, a.c.cap) + a.chunk - 1) / a.chunk;
+    const size_t rh = (size_t)row * a.hQ + h, at = rh * a.n_split;
+    float m = AR_FLOOR, l = 0.f;
+    if (lane < n) {
+        m = a.ml[2 * (at + lane)];
+        l = a.ml[2 * (at + lane) + 1];
+    }
+    // exp2 of a difference of maxima: NaN where a range saw one, which the sums below carry on
+    const float top = wave_max(m), f = lane < n ? __builtin_amdgcn_exp2f(m - top) : 0.f;
+    const float sum = wave_sum(l * f);
+    float o[PER];
+#pragma unroll
+    for (uint32_t e = 0; e < PER; e++) o[e] = 0.f;
+    for (uint32_t s0 = 0; s0 < n; s0 += 8) {
+        float x[8][PER];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++)
+#pragma unroll
+            for (uint32_t e = 0; e < PER; e++) x[i][e] = a.acc[(at + min(s0 + i, n - 1)) * DH + PER * lane + e];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            const float w = __shfl(f, (int)min(s0 + i, 63u));
+#pragma unroll
+            for (uint32_t e = 0; e < PER; e++)
+                if (s0 + i < n) o[e] += x[i][e] * w;
+        }
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < PER; e++) {
+        float v = sum == 0.f ? 0.f : o[e] / sum;
+        if (a.qfull) v *= 1.f / (1.f + expf(-a.qfull[rh * 2 * DH + DH + PER * lane + e]));
+        a.att[rh * DH + PER * lane + e] = v;
+    }
+}
+
+// How a call is cut, from what the host knows (never from the lengths, which live on the device, so that a captured launch
+// follows them): which kernel, and the ranges of keys that run in parallel.
+struct Plan {
+    bool few;
+    uint32_t n_split, chunk;
+};
+static Plan plan_of(const qkk_kv_cache* C, const qkk_kv_runs* R, uint32_t hQ)
+{
+    const uint32_t G = hQ / C->n_kv, max_run = std::min(R->max_run, R->n_rows);
+    const uint64_t cap = (uint64_t)C->seq_pages * C->page_rows;
+    Plan p;
+    p.few = (uint64_t)max_run * G <= few_rows(C->dh);
+    if (!p.few) return Plan{false, 1, (uint32_t)cap};
+    // ranges of 128 keys (a step per wave) while about a thousand workgroups cover the whole cache with them, longer ones beyond;
+    // at most 64 (the join's lanes)
+    const uint64_t units = (uint64_t)R->n_run * C->n_kv;
+    const uint64_t want = std::max((cap * units + 1023) / 1024, (cap + 63) / 64);
+    p.chunk = (uint32_t)std::max<uint64_t>(128, (want + 127) / 128 * 128);
+    p.n_split = (uint32_t)((cap + p.chunk - 1) / p.chunk);
+    return p;
+}
+
 static int attn_runs(const char* who, const qkk_kv_cache* C, uint32_t layer, const qkk_kv_runs* R, const int32_t* parent, bool tree,
                      const float* qhat, const float* qfull, float* att, void* workspace, size_t workspace_bytes, uint32_t hQ, void* stream)
 {
@@ -103,6 +173,31 @@ static int attn_runs(const char* who, const qkk_kv_cache* C, uint32_t layer, con
     if (workspace_bytes < want) return fail(QKK_EWORKSPACE, "%s: workspace %zu < %zu bytes", who, workspace_bytes, want);
     if (int rc = require_device()) return rc;
     if (!runs.n_rows || !runs.n_run) return QKK_OK;
+    const Plan plan = plan_of(C, R, hQ);
+    if ((uint64_t)runs.n_run * c.n_kv * plan.n_split > (1u << 30) || (uint64_t)runs.n_rows * hQ > (1u << 30))
+        return fail(QKK_ESHAPE, "%s: rows x heads or runs x heads too large", who);
+    if (plan.few) {
+        RunsCall a;
+        a.c = c;
+        a.R = runs;
+        a.parent = parent;
+        a.q = qhat;
+        a.qfull = qfull;
+        a.att = att;
+        a.acc = (float*)workspace;
+        a.ml = a.acc + (size_t)runs.n_rows * hQ * plan.n_split * C->dh;
+        a.hQ = hQ;
+        a.G = hQ / c.n_kv;
+        a.n_split = plan.n_split;
+        a.chunk = plan.chunk;
+        launch_attn_few(a, C->type, C->dh, tree, as_stream(stream));
+        if (plan.n_split > 1) {
+            const dim3 jobs((uint32_t)(((uint64_t)runs.n_rows * hQ + 3) / 4));
+            if (C->dh == 256) hipLaunchKernelGGL(attn_join_kernel<256>, jobs, dim3(256), 0, as_stream(stream), a);
+            else hipLaunchKernelGGL(attn_join_kernel<128>, jobs, dim3(256), 0, as_stream(stream), a);
+        }
+        return check_launch(who);
+    }
     const dim3 grid(runs.n_rows, hQ), block(256);
 #define QK_RUNS(DH, T, TREE)                                                                                                             \
     hipLaunchKernelGGL((attn_runs_plain_kernel<DH, T, TREE>), grid, block, 0, as_stream(stream), c, runs, parent, qhat, qfull, att, hQ)
@@ -127,8 +222,9 @@ extern "C" {
 
 size_t qkk_attn_runs_workspace_bytes(const qkk_kv_cache* C, const qkk_kv_runs* R, uint32_t hQ)
 {
-    if (!C || !R || !hQ) return 0;
-    return 256;
+    if (!C || !R || !C->n_kv || hQ < C->n_kv || !C->seq_pages || !C->page_rows) return 0;
+    const Plan p = plan_of(C, R, hQ);
+    return (p.n_split > 1 ? (size_t)R->n_rows * hQ * p.n_split * (C->dh + 2) * sizeof(float) : 0) + 256;
 }
 
 int qkk_attn_packed(const qkk_kv_cache* C, uint32_t layer, const qkk_kv_runs* R, const float* qhat, const float* qfull, float* att,

@@ -426,14 +426,15 @@ Graph* capture_end()
 
 } // namespace emu
 
-emu_float4 emu_mfma_16x16x32_f16(emu_half8 a, emu_half8 b, emu_float4 c)
+// the sums of a 16x16x32 product from the lanes' operands, widened to float
+static emu_float4 mfma_16x16x32(const float* a, const float* b, emu_float4 c)
 {
     using namespace emu;
     Workgroup& g = *t_wg;
     const uint32_t t = g.cur->tid.x, w = t >> 6, lane = t & 63u, par = g.cur->xn++ & 1u;
     for (int i = 0; i < 8; i++) {
-        g.mfma_a[w][par][lane][i] = (float)a[i];
-        g.mfma_b[w][par][lane][i] = (float)b[i];
+        g.mfma_a[w][par][lane][i] = a[i];
+        g.mfma_b[w][par][lane][i] = b[i];
     }
     wave_barrier();
     const uint32_t col = lane & 15u, rq = lane >> 4;
@@ -446,6 +447,28 @@ emu_float4 emu_mfma_16x16x32_f16(emu_half8 a, emu_half8 b, emu_float4 c)
         d[i] += s;
     }
     return d;
+}
+emu_float4 emu_mfma_16x16x32_f16(emu_half8 a, emu_half8 b, emu_float4 c)
+{
+    float x[8], y[8];
+    for (int i = 0; i < 8; i++) {
+        x[i] = (float)a[i];
+        y[i] = (float)b[i];
+    }
+    return mfma_16x16x32(x, y, c);
+}
+emu_float4 emu_mfma_16x16x32_bf16(emu_bf16x8 a, emu_bf16x8 b, emu_float4 c)
+{
+    uint16_t ah[8], bh[8];
+    float x[8], y[8];
+    memcpy(ah, &a, 16);
+    memcpy(bh, &b, 16);
+    for (int i = 0; i < 8; i++) {
+        const uint32_t u = (uint32_t)ah[i] << 16, v = (uint32_t)bh[i] << 16;
+        memcpy(&x[i], &u, 4);
+        memcpy(&y[i], &v, 4);
+    }
+    return mfma_16x16x32(x, y, c);
 }
 
 // Device allocations of the library itself (the engine's tensors): guarded like the tests' buffers.

@@ -291,6 +291,9 @@ static inline uint32_t emu_perm(uint32_t s0, uint32_t s1, uint32_t sel)
 typedef _Float16 emu_half8 __attribute__((ext_vector_type(8)));
 typedef float emu_float4 __attribute__((ext_vector_type(4)));
 emu_float4 emu_mfma_16x16x32_f16(emu_half8 a, emu_half8 b, emu_float4 c);
+// v_mfma_f32_16x16x32_bf16: the same lanes with bfloat16 operands
+typedef __bf16 emu_bf16x8 __attribute__((ext_vector_type(8)));
+emu_float4 emu_mfma_16x16x32_bf16(emu_bf16x8 a, emu_bf16x8 b, emu_float4 c);
 
 #define __builtin_amdgcn_update_dpp emu_update_dpp
 #define __builtin_amdgcn_readlane emu_readlane
@@ -301,6 +304,8 @@ emu_float4 emu_mfma_16x16x32_f16(emu_half8 a, emu_half8 b, emu_float4 c);
 #define __builtin_amdgcn_perm emu_perm
 #define __builtin_amdgcn_cvt_pkrtz emu_cvt_pkrtz
 #define __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, x, y, z) emu_mfma_16x16x32_f16(a, b, c)
+#define __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, x, y, z) emu_mfma_16x16x32_bf16(a, b, c)
+#define __builtin_amdgcn_exp2f(x) exp2f(x)
 #define __builtin_amdgcn_s_waitcnt(x) ((void)0)
 #define __builtin_amdgcn_sched_barrier(x) ((void)0)
 #define __builtin_amdgcn_sched_group_barrier(a, b, c) ((void)0)
