@@ -169,7 +169,11 @@ def _ptr(t):
 
 
 def _stream():
+    """The current stream of the current device as a C pointer."""
     import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # the handle itself: a tenth of the time of building a Stream object
+    if raw is not None:
+        return C.c_void_p(raw(torch.cuda.current_device()))
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
@@ -557,22 +561,27 @@ def dn_step(conv, gb, state, norm_w, z, hK, hV, kdiv=0, d_state=128, eps=1e-6, a
 
 # ---- the paged cache and the attention over runs of rows ------------------------------------------
 
-def _want(who, device, **tensors):
-    """Each named (tensor, dtype, shape or None): on the device of the cache, contiguous, of that type and shape."""
-    for name, (t, dtype, shape) in tensors.items():
-        if t is None:
-            continue
-        if t.device != device or t.dtype != dtype or not t.is_contiguous() or (shape is not None and tuple(t.shape) != tuple(shape)):
-            raise ValueError(f"{who}: {name} must be a contiguous {dtype} tensor" + (f" of shape {tuple(shape)}" if shape is not None else "") +
-                             f" on {device}, not {t.dtype} {tuple(t.shape)} on {t.device}" + ("" if t.is_contiguous() else " (strided)"))
+def _want(who, name, t, dtype, shape, dev):
+    """t: a contiguous tensor of that type and shape (None: any) on device number `dev` (-1: host memory), or ValueError.  Cheap: a
+    decode step makes these checks for every layer."""
+    if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous() or (shape is not None and t.shape != shape):
+        raise ValueError(f"{who}: {name} must be a contiguous {dtype} tensor" + (f" of shape {tuple(shape)}" if shape is not None else "") +
+                         f" on device {dev}, not {t.dtype} {tuple(t.shape)} on {t.get_device()}" + ("" if t.is_contiguous() else " (strided)"))
+    return t.data_ptr()
 
 
-def _here(who, device):
-    """The calls go to the current device's current stream: the cache has to be there."""
-    if device.type == "cuda":
+def _here(who, dev):
+    """The calls go to the current device's current stream: the cache has to be there.  Returns that stream."""
+    if dev >= 0:
         import torch
-        if device.index != torch.cuda.current_device():
-            raise ValueError(f"{who}: the cache is on {device}, the current device is cuda:{torch.cuda.current_device()}")
+        if dev != torch.cuda.current_device():
+            raise ValueError(f"{who}: the cache is on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
+    return _stream()
+
+
+def _bytes(who, t, dev):
+    """(address, bytes) of a workspace."""
+    return _want(who, "workspace", t, t.dtype, None, dev), t.numel() * t.element_size()
 
 
 class KvCache:
@@ -582,6 +591,7 @@ class KvCache:
 
     def __init__(self, k, v, table=None, ref=None, len=None, n_seq=None):
         import torch
+        self.f32, self.i32, self.u8 = torch.float32, torch.int32, torch.uint8
         types = {torch.float32: F32, torch.float16: F16}
         if k.dim() != 5 or k.dtype not in types:
             raise ValueError("KvCache: k must be a float32 or float16 tensor [n_layer][n_page][n_kv][page_rows][dh]")
@@ -592,9 +602,11 @@ class KvCache:
             n_seq, seq_pages = table.shape
         else:
             n_seq, seq_pages = n_page if n_seq is None else n_seq, 1
-        i32 = torch.int32
-        _want("KvCache", k.device, k=(k, k.dtype, None), v=(v, k.dtype, k.shape), table=(table, i32, None), ref=(ref, i32, (n_page,)),
-              len=(len, i32, (n_seq,)))
+        self.dev = k.get_device()
+        for name, t, dtype, shape in (("k", k, k.dtype, None), ("v", v, k.dtype, k.shape), ("table", table, self.i32, None),
+                                      ("ref", ref, self.i32, (n_page,)), ("len", len, self.i32, (n_seq,))):
+            if t is not None:
+                _want("KvCache", name, t, dtype, shape, self.dev)
         self.k, self.v, self.table, self.ref, self.len = k, v, table, ref, len
         self.n_layer, self.n_page, self.n_kv, self.page_rows, self.dh = n_layer, n_page, n_kv, page_rows, dh
         self.n_seq, self.seq_pages, self.device = n_seq, seq_pages, k.device
@@ -609,11 +621,11 @@ class KvRuns:
     run is longer (default n_rows)."""
 
     def __init__(self, n_rows, start, seq, pos, max_run=None):
+        n_run, dev = seq.numel(), seq.get_device()
         import torch
-        n_run = seq.numel()
-        i32 = torch.int32
-        _want("KvRuns", seq.device, seq=(seq, i32, (n_run,)), start=(start, i32, (n_run + 1,)), pos=(pos, i32, (n_run,)))
-        self.start, self.seq, self.pos, self.n_rows, self.n_run, self.device = start, seq, pos, n_rows, n_run, seq.device
+        for name, t, n in (("seq", seq, n_run), ("start", start, n_run + 1), ("pos", pos, n_run)):
+            _want("KvRuns", name, t, torch.int32, (n,), dev)
+        self.start, self.seq, self.pos, self.n_rows, self.n_run, self.dev = start, seq, pos, n_rows, n_run, dev
         self.max_run = n_rows if max_run is None else max_run
         self.c = _KvRuns(n_rows, n_run, self.max_run, start.data_ptr(), seq.data_ptr(), pos.data_ptr())
         self.ref_c = C.byref(self.c)
@@ -629,24 +641,32 @@ def rope_axes(n_rot, sections, in_turn=False):
     return out
 
 
+def _same_device(who, cache, runs):
+    if runs.dev != cache.dev:
+        raise ValueError(f"{who}: the runs are on device {runs.dev}, the cache on {cache.dev}")
+
+
 def attn_prep_axes(cache, layer, runs, q, kin, vin, q_norm_w, k_norm_w, rope, pair_axis, axis_pos, eps=1e-6, qhat=None):
     """Head norm, rotation with several position axes, cache write for the rows of runs.  q [rows][hQ][dh], or [rows][hQ][2*dh] with
     the output gate behind each head's query; kin / vin [rows][n_kv][dh]; rope [rope_rows][n_rot/2][2]; pair_axis uint8
     [n_rot/2]; axis_pos int32 [n_axis][rows].  Returns qhat [rows][hQ][dh]."""
-    import torch
-    f, rows, dh = torch.float32, runs.n_rows, cache.dh
-    hQ = q.shape[1] if q.dim() == 3 else 0
-    if q.dim() != 3 or q.shape[2] not in (dh, 2 * dh) or rope.dim() != 3 or rope.shape[2] != 2 or axis_pos.dim() != 2:
+    who, f, rows, dh, dev = "attn_prep_axes", cache.f32, runs.n_rows, cache.dh, cache.dev
+    if q.dim() != 3 or rope.dim() != 3 or rope.shape[2] != 2 or axis_pos.dim() != 2 or q.shape[2] not in (dh, 2 * dh):
         raise ValueError("attn_prep_axes: q must be [rows][hQ][dh or 2*dh], rope [rope_rows][n_rot/2][2], axis_pos [n_axis][rows]")
-    _here("attn_prep_axes", cache.device)
+    _, hQ, pitch = q.shape
+    rope_rows, half, _ = rope.shape
+    n_axis = axis_pos.shape[0]
+    stream = _here(who, dev)
+    _same_device(who, cache, runs)
     if qhat is None:
-        qhat = torch.empty((rows, hQ, dh), dtype=f, device=q.device)
-    _want("attn_prep_axes", cache.device, start=(runs.start, torch.int32, None), q=(q, f, (rows, hQ, q.shape[2])), kin=(kin, f, (rows, cache.n_kv, dh)),
-          vin=(vin, f, (rows, cache.n_kv, dh)), q_norm_w=(q_norm_w, f, (dh,)), k_norm_w=(k_norm_w, f, (dh,)), rope=(rope, f, None),
-          pair_axis=(pair_axis, torch.uint8, (rope.shape[1],)), axis_pos=(axis_pos, torch.int32, (axis_pos.shape[0], rows)), qhat=(qhat, f, (rows, hQ, dh)))
-    _check(lib().qkk_attn_prep_axes(cache.ref_c, layer, runs.ref_c, _ptr(q), _ptr(kin), _ptr(vin), _ptr(q_norm_w), _ptr(k_norm_w), _ptr(rope),
-                                    rope.shape[0], _ptr(pair_axis), axis_pos.shape[0], _ptr(axis_pos), _ptr(qhat), hQ, 2 * rope.shape[1],
-                                    int(q.shape[2] != dh), eps, _stream()))
+        qhat = q.new_empty((rows, hQ, dh))
+    kv, w = (rows, cache.n_kv, dh), (dh,)
+    _check(lib().qkk_attn_prep_axes(
+        cache.ref_c, layer, runs.ref_c, _want(who, "q", q, f, (rows, hQ, pitch), dev), _want(who, "kin", kin, f, kv, dev),
+        _want(who, "vin", vin, f, kv, dev), _want(who, "q_norm_w", q_norm_w, f, w, dev), _want(who, "k_norm_w", k_norm_w, f, w, dev),
+        _want(who, "rope", rope, f, None, dev), rope_rows, _want(who, "pair_axis", pair_axis, cache.u8, (half,), dev), n_axis,
+        _want(who, "axis_pos", axis_pos, cache.i32, (n_axis, rows), dev), _want(who, "qhat", qhat, f, (rows, hQ, dh), dev), hQ, 2 * half,
+        int(pitch != dh), eps, stream))
     return qhat
 
 
@@ -655,22 +675,23 @@ def attn_runs_workspace_bytes(cache, runs, hQ):
 
 
 def _attn_runs(who, cache, layer, runs, parent, qhat, workspace, qfull, att):
-    import torch
-    f, rows = torch.float32, runs.n_rows
+    f, rows, dev, dh = cache.f32, runs.n_rows, cache.dev, cache.dh
     if qhat.dim() != 3:
         raise ValueError(f"{who}: qhat must be [rows][hQ][dh]")
-    hQ, dh = qhat.shape[1], cache.dh
-    _here(who, cache.device)
+    hQ = qhat.shape[1]
+    stream = _here(who, dev)
+    _same_device(who, cache, runs)
     if att is None:
-        att = torch.empty_like(qhat)
-    _want(who, cache.device, start=(runs.start, torch.int32, None), qhat=(qhat, f, (rows, hQ, dh)), att=(att, f, (rows, hQ, dh)),
-          qfull=(qfull, f, (rows, hQ, 2 * dh)), parent=(parent, torch.int32, (rows,)), workspace=(workspace, workspace.dtype, None))
-    nbytes = workspace.numel() * workspace.element_size()
+        att = qhat.new_empty((rows, hQ, dh))
+    shape = (rows, hQ, dh)
+    q, out = _want(who, "qhat", qhat, f, shape, dev), _want(who, "att", att, f, shape, dev)
+    gate = 0 if qfull is None else _want(who, "qfull", qfull, f, (rows, hQ, 2 * dh), dev)
+    space, nbytes = _bytes(who, workspace, dev)
     if parent is None:
-        _check(lib().qkk_attn_packed(cache.ref_c, layer, runs.ref_c, _ptr(qhat), _ptr(qfull), _ptr(att), _ptr(workspace), nbytes, hQ, _stream()))
+        _check(lib().qkk_attn_packed(cache.ref_c, layer, runs.ref_c, q, gate, out, space, nbytes, hQ, stream))
     else:
-        _check(lib().qkk_attn_tree(cache.ref_c, layer, runs.ref_c, _ptr(parent), _ptr(qhat), _ptr(qfull), _ptr(att), _ptr(workspace), nbytes, hQ,
-                                   _stream()))
+        up = _want(who, "parent", parent, cache.i32, (rows,), dev)
+        _check(lib().qkk_attn_tree(cache.ref_c, layer, runs.ref_c, up, q, gate, out, space, nbytes, hQ, stream))
     return att
 
 
@@ -692,44 +713,39 @@ def kv_workspace_bytes(cache):
     return lib().qkk_kv_workspace_bytes(cache.ref_c)
 
 
-def _status(who, cache, status, workspace):
-    import torch
-    _here(who, cache.device)
-    if status is None:
-        status = torch.empty(1, dtype=torch.int32, device=cache.device)
-    _want(who, cache.device, status=(status, torch.int32, (1,)), workspace=(workspace, workspace.dtype, None))
-    return status
-
-
 def kv_resize(cache, len_new, workspace, status=None):
     """Sets the rows each sequence holds (int32 [n_seq]; -1: as it is, 0: freed); pages are freed and taken, a shared part-filled page is
     copied before its sequence grows.  Returns the device status word: 0, the number of missing pages (nothing grew), or -1."""
-    import torch
-    status = _status("kv_resize", cache, status, workspace)
-    _want("kv_resize", cache.device, len_new=(len_new, torch.int32, (cache.n_seq,)))
-    _check(lib().qkk_kv_resize(cache.ref_c, _ptr(len_new), _ptr(status), _ptr(workspace), workspace.numel() * workspace.element_size(), _stream()))
+    who, dev = "kv_resize", cache.dev
+    stream = _here(who, dev)
+    if status is None:
+        status = len_new.new_empty((1,))
+    space, nbytes = _bytes(who, workspace, dev)
+    _check(lib().qkk_kv_resize(cache.ref_c, _want(who, "len_new", len_new, cache.i32, (cache.n_seq,), dev),
+                               _want(who, "status", status, cache.i32, (1,), dev), space, nbytes, stream))
     return status
 
 
 def kv_fork(cache, src, dst, workspace, status=None):
     """Sequences dst (empty) get the rows of src, sharing their pages (a slot cache: copies of the rows).  Returns the device status
     word: 0, or -1 where nothing was changed."""
-    import torch
-    status = _status("kv_fork", cache, status, workspace)
-    n = src.numel()
-    _want("kv_fork", cache.device, src=(src, torch.int32, (n,)), dst=(dst, torch.int32, (n,)))
-    _check(lib().qkk_kv_fork(cache.ref_c, _ptr(src), _ptr(dst), n, _ptr(status), _ptr(workspace), workspace.numel() * workspace.element_size(),
-                             _stream()))
+    who, dev, n = "kv_fork", cache.dev, src.numel()
+    stream = _here(who, dev)
+    if status is None:
+        status = src.new_empty((1,))
+    space, nbytes = _bytes(who, workspace, dev)
+    _check(lib().qkk_kv_fork(cache.ref_c, _want(who, "src", src, cache.i32, (n,), dev), _want(who, "dst", dst, cache.i32, (n,), dev), n,
+                             _want(who, "status", status, cache.i32, (1,), dev), space, nbytes, stream))
     return status
 
 
 def kv_compact(cache, seq, base, path, n_path):
     """Moves the accepted rows base + path[i][j] of sequence seq[i] to base + j, j < n_path[i], in all layers; path int32 [n][max_path],
     ascending per path."""
-    import torch
-    i32, n = torch.int32, seq.numel()
+    who, dev, i32, n = "kv_compact", cache.dev, cache.i32, seq.numel()
     if path.dim() != 2:
         raise ValueError("kv_compact: path must be [n][max_path]")
-    _here("kv_compact", cache.device)
-    _want("kv_compact", cache.device, seq=(seq, i32, (n,)), base=(base, i32, (n,)), path=(path, i32, (n, path.shape[1])), n_path=(n_path, i32, (n,)))
-    _check(lib().qkk_kv_compact(cache.ref_c, _ptr(seq), _ptr(base), _ptr(path), _ptr(n_path), n, path.shape[1], _stream()))
+    stream = _here(who, dev)
+    wide = path.shape[1]
+    _check(lib().qkk_kv_compact(cache.ref_c, _want(who, "seq", seq, i32, (n,), dev), _want(who, "base", base, i32, (n,), dev),
+                                _want(who, "path", path, i32, (n, wide), dev), _want(who, "n_path", n_path, i32, (n,), dev), n, wide, stream))

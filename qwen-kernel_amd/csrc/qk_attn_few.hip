@@ -1,14 +1,17 @@
 // qk_attn_few.hip -- attention of runs with FEW query rows (one or two blocks of 16 per run and KV head: decode steps, small trees) over
 // the paged cache.  Bound by reading the cache, which every run does once per KV head.
 //
-// A workgroup takes one run, one KV head and one range of keys; its four waves take the range's steps of 32 keys in turn.
-// A wave loads the A operands of both products straight from the cache into registers, nothing goes through LDS:
+// A workgroup takes one run, one KV head and one range of keys; its four waves take the range's steps in turn, 32 keys or (half
+// cache, dh 128) 64.  A wave loads the A operands of both products straight from the cache into registers, nothing goes
+// through LDS:
 //   K  lane (m, g) holds 8 dims per step of 32 dims of key m (rows of the S^T block);
 //   V  lane (m, g) holds, of the 8 keys that its P covers, 4 (fp32) or 8 (half) NEIGHBOURING dims: which dims a block of 16
 //      rows of O^T stands for is free, so block e of a group takes dim E*m + e of lane m, and loads stay 16 bytes wide, 256
 //      bytes side by side, without a transposition.
-// A step is four pieces of at most 16 KB -- the K of either block of 16 keys, V in two halves -- and each is requested as
-// soon as the piece two places before it has been used, into its registers: 16 to 32 KB are on the way per wave.
+// A step is 32 KB per wave in flight: its K and V are requested together, the next step's K when this one's scores are done and
+// its V when this one's values are.  Only fp32 with dh 256, where a step is 64 KB, requests V in two halves behind the two
+// halves of K (registers).  What a launch of a few steps per wave spends is the chain of round trips: run -> page table -> keys;
+// queries and parents are requested before the keys and prepared while those arrive.
 // An fp32 cache is split into three bf16 pieces in registers (exact, fp32's whole range, NaN and infinities stay in their
 // key), six of the nine products are kept (the others are below 2^-23 of their terms); a half cache is an operand as it is,
 // and queries and weights go in as hi + lo halves: two products.  Matrix work is a few percent of the time either way.
@@ -18,9 +21,10 @@ namespace qk {
 
 typedef u32x4 __attribute__((may_alias)) lds_u32x4;
 typedef f32x4 __attribute__((may_alias)) lds_f32x4;
+typedef uint32_t __attribute__((may_alias)) lds_pair;
 
 template <int DH, bool F32, int RT, bool TREE>
-__global__ __launch_bounds__(256, 1) void attn_few_kernel(RunsCall a)
+__global__ __launch_bounds__(256, (DH == 128 && RT == 1 ? 2 : 1)) void attn_few_kernel(RunsCall a)
 {
     constexpr uint32_t KS = DH / 32;            // steps of 32 dims
     constexpr uint32_t E = F32 ? 4 : 8;         // neighbouring dims a lane loads
@@ -33,26 +37,90 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(RunsCall a)
     __shared__ int32_t s_up[TREE ? QKK_TREE_MAX : 1];
     __shared__ uint32_t s_kin[TREE ? RT * 16 : 1][QKK_TREE_MAX / 32];
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, m = lane & 15u, g = lane >> 4;
-    const uint32_t split = blockIdx.x % a.n_split, kv = blockIdx.x / a.n_split % a.c.n_kv, run = blockIdx.x / a.n_split / a.c.n_kv;
+    // Workgroups go to the eight dies in turn, so the KV head and the run vary fastest: every die gets the same share of the first
+    // ranges, which every run has, and of the last ones, which few have (with the range varying fastest one die had all the first).
+    const uint32_t kv = blockIdx.x % a.c.n_kv, run = blockIdx.x / a.c.n_kv % a.R.n_run, split = blockIdx.x / a.c.n_kv / a.R.n_run;
     const Run u = run_at(a.c, a.R, run);
     const uint32_t nr = u.n * a.G, end = min(u.pos + u.n, a.c.cap), k_begin = split * a.chunk;
     if (!u.ok || nr == 0 || k_begin >= end) return; // the whole workgroup
     const uint32_t k_end = min(end, k_begin + a.chunk);
     const bool drafts = TREE && k_end > u.pos; // uniform: this range holds rows of the tree itself
-    if (drafts) tree_bits(a.parent, u, 0, u.n, s_up, s_kin);
+    int32_t up_of = -1;
+    if (drafts) up_of = tree_parent(a.parent, u);
 
     // Q: wave w prepares rows 4 RT w .. 4 RT w + 4 RT - 1, a lane PER neighbouring dims
     constexpr uint32_t PER = DH / 64;
-    float q_exp[RT]; // 2^exponent the lane's row was divided by (half caches)
-    {
-        float x[4 * RT][PER];
+    float qx[4 * RT][PER];
 #pragma unroll
-        for (uint32_t i = 0; i < 4 * RT; i++) {
-            const uint32_t f = 4 * RT * wave + i;
+    for (uint32_t i = 0; i < 4 * RT; i++) {
+        const uint32_t f = 4 * RT * wave + i;
 #pragma unroll
-            for (uint32_t j = 0; j < PER; j++)
-                x[i][j] = f < nr ? a.q[((size_t)(u.r0 + f / a.G) * a.hQ + kv * a.G + f % a.G) * DH + PER * lane + j] : 0.f;
+        for (uint32_t j = 0; j < PER; j++)
+            qx[i][j] = f < nr ? a.q[((size_t)(u.r0 + f / a.G) * a.hQ + kv * a.G + f % a.G) * DH + PER * lane + j] : 0.f;
+    }
+
+    // one step's operands: K [sub-step of 32 keys][block of 16 keys][step of 32 dims], V [sub-step][group][key of the lane's 8]
+    constexpr uint32_t SUB = !F32 && DH == 128 ? 2 : 1, SK = 32 * SUB; // sub-steps, keys per step
+    constexpr uint32_t KW = F32 ? 2 : 1;                               // 16-byte pieces per lane, block and step of dims
+    constexpr bool HALVES = F32 && DH == 256;                          // V in two halves, behind those of K
+    constexpr uint32_t CA = HALVES ? NC / 2 : NC;                      // groups of V's first part
+    const uint32_t n_step = (k_end - k_begin + SK - 1) / SK;
+    u32x4 kreg[SUB][2][KS][KW], vreg[SUB][NC][8];
+    const u32x4 zero = {0, 0, 0, 0};
+    const uint8_t* kbase = (const uint8_t*)a.c.k;
+    const uint8_t* vbase = (const uint8_t*)a.c.v;
+    constexpr uint32_t ES = F32 ? 4 : 2;
+    // the pages of a step's blocks of 16 keys (a page holds a multiple of 16 rows; a slot cache is one page)
+    auto pages = [&](uint32_t step, uint32_t* pg) {
+#pragma unroll
+        for (uint32_t b = 0; b < 2 * SUB; b++) {
+            const uint32_t key = k_begin + SK * step + 16 * b;
+            pg[b] = key < k_end ? kv_page(a.c, u.seq, key) : KV_NO_PAGE;
         }
+    };
+    // block b of K.  Rows behind the range repeat its last one (masked below); without a page, and behind the last step: zeros, no load
+    auto fetch_k = [&](uint32_t step, uint32_t b, const uint32_t* pg) {
+        const uint32_t key = min(k_begin + SK * step + 16 * b + m, k_end - 1);
+        if (pg[b] != KV_NO_PAGE) { // uniform
+            const uint8_t* row = kbase + kv_row(a.c, pg[b], kv, key, DH) * ES;
+#pragma unroll
+            for (uint32_t ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (uint32_t w = 0; w < KW; w++) kreg[b / 2][b % 2][ks][w] = *(const u32x4*)(row + (F32 ? ks * 128 + w * 64 : ks * 64) + g * 16);
+        } else {
+#pragma unroll
+            for (uint32_t ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (uint32_t w = 0; w < KW; w++) kreg[b / 2][b % 2][ks][w] = zero;
+        }
+    };
+    // groups c0 .. c1 - 1 of sub-step sb of V
+    auto fetch_v = [&](uint32_t step, uint32_t sb, uint32_t c0, uint32_t c1, const uint32_t* pg) {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            const uint32_t b = 2 * sb + i / 4, key = min(k_begin + SK * step + 16 * b + 4 * g + i % 4, k_end - 1);
+            if (pg[b] != KV_NO_PAGE) { // uniform
+                const uint8_t* row = vbase + kv_row(a.c, pg[b], kv, key, DH) * ES;
+#pragma unroll
+                for (uint32_t c = c0; c < c1; c++) vreg[sb][c][i] = *(const u32x4*)(row + (c * 16 + m) * 16);
+            } else {
+#pragma unroll
+                for (uint32_t c = c0; c < c1; c++) vreg[sb][c][i] = zero;
+            }
+        }
+    };
+    uint32_t pg[2 * SUB], pg_next[2 * SUB];
+    pages(wave, pg);
+    __builtin_amdgcn_sched_barrier(0); // the queries are on their way before the keys
+#pragma unroll
+    for (uint32_t b = 0; b < 2 * SUB; b++) fetch_k(wave, b, pg);
+    if (!HALVES) {
+#pragma unroll
+        for (uint32_t sb = 0; sb < SUB; sb++) fetch_v(wave, sb, 0, NC, pg);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
+    {
         uint16_t* s_q = (uint16_t*)s_dyn;
         const uint32_t d = PER * lane, ks = d / 32, in = d % 32;
         // the lane group and the place among its 8 values that hold dim `in` of a step
@@ -64,37 +132,43 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(RunsCall a)
             if (!F32) {
                 float mx = 0.f;
 #pragma unroll
-                for (uint32_t j = 0; j < PER; j++) mx = fmaxf(mx, fabsf(x[i][j]));
+                for (uint32_t j = 0; j < PER; j++) mx = fmaxf(mx, fabsf(qx[i][j]));
                 mx = wave_max(mx);
                 const int e = top_exponent(mx);
                 scale = pow2i(-e);
                 if (lane == 0) s_m[0][f] = pow2i(e);
             }
+            uint16_t bits[NP][PER];
 #pragma unroll
             for (uint32_t j = 0; j < PER; j++) {
-                float v = x[i][j] * scale;
+                float v = qx[i][j] * scale;
 #pragma unroll
                 for (uint32_t p = 0; p < NP; p++) {
-                    uint16_t bits;
                     if (F32) {
-                        bits = (uint16_t)(f2u(v) >> 16);
+                        bits[p][j] = (uint16_t)(f2u(v) >> 16);
                         v -= u2f(f2u(v) & 0xFFFF0000u);
                     } else {
                         const _Float16 hv = (_Float16)v;
-                        bits = __builtin_bit_cast(uint16_t, hv);
+                        bits[p][j] = __builtin_bit_cast(uint16_t, hv);
                         v -= (float)hv;
                     }
-                    s_q[(((p * RT + rt) * KS + ks) * 64 + 16 * qg + f % 16) * 8 + qt + j] = bits;
                 }
+            }
+#pragma unroll
+            for (uint32_t p = 0; p < NP; p++) {
+                uint16_t* at = s_q + (((p * RT + rt) * KS + ks) * 64 + 16 * qg + f % 16) * 8 + qt;
+#pragma unroll
+                for (uint32_t j = 0; j < PER; j += 2) *(lds_pair*)(at + j) = (uint32_t)bits[p][j] | (uint32_t)bits[p][j + 1] << 16;
             }
         }
     }
+    if (drafts) tree_bits(up_of, 0, u.n, s_up, s_kin);
     __syncthreads();
+    float q_exp[RT]; // 2^exponent the lane's row was divided by (half caches)
 #pragma unroll
     for (uint32_t rt = 0; rt < RT; rt++) q_exp[rt] = F32 ? 1.f : s_m[0][16 * rt + m];
     const lds_u32x4* q_op = (const lds_u32x4*)s_dyn;
 
-    const uint32_t n_step = (k_end - k_begin + 31) / 32;
     const float qs = AR_LOG2E / sqrtf((float)DH);
     float4v o[RT][NT];
     float m_run[RT], l_run[RT];
@@ -105,74 +179,22 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(RunsCall a)
 #pragma unroll
         for (uint32_t t = 0; t < NT; t++) o[rt][t] = float4v{0.f, 0.f, 0.f, 0.f};
     }
-    // one step's operands: K [block of 16 keys][step of 32 dims], V [group][key of the lane's 8]
-    constexpr uint32_t KW = F32 ? 2 : 1; // 16-byte pieces per lane, block and step
-    constexpr uint32_t CA = (NC + 1) / 2; // groups of V's first piece
-    u32x4 kreg[2][KS][KW], vreg[NC][8];
-    const u32x4 zero = {0, 0, 0, 0};
-    const uint8_t* kbase = (const uint8_t*)a.c.k;
-    const uint8_t* vbase = (const uint8_t*)a.c.v;
-    constexpr uint32_t ES = F32 ? 4 : 2;
-    // the pages of a step's two blocks of 16 keys (a page holds a multiple of 16 rows; a slot cache is one page)
-    auto pages = [&](uint32_t step, uint32_t* pg) {
-#pragma unroll
-        for (uint32_t b = 0; b < 2; b++) {
-            const uint32_t key = k_begin + 32 * step + 16 * b;
-            pg[b] = key < k_end ? kv_page(a.c, u.seq, key) : KV_NO_PAGE;
-        }
-    };
-    auto fetch_k = [&](uint32_t step, uint32_t b, const uint32_t* pg) {
-        {
-            const uint32_t key = min(k_begin + 32 * step + 16 * b + m, k_end - 1); // rows behind the range repeat its last one, masked below
-            if (pg[b] != KV_NO_PAGE) { // uniform
-                const uint8_t* row = kbase + kv_row(a.c, pg[b], kv, key, DH) * ES;
-#pragma unroll
-                for (uint32_t ks = 0; ks < KS; ks++)
-#pragma unroll
-                    for (uint32_t w = 0; w < KW; w++) kreg[b][ks][w] = *(const u32x4*)(row + (F32 ? ks * 128 + w * 64 : ks * 64) + g * 16);
-            } else {
-#pragma unroll
-                for (uint32_t ks = 0; ks < KS; ks++)
-#pragma unroll
-                    for (uint32_t w = 0; w < KW; w++) kreg[b][ks][w] = zero;
-            }
-        }
-    };
-    auto fetch_v = [&](uint32_t step, uint32_t c0, uint32_t c1, const uint32_t* pg) {
-#pragma unroll
-        for (uint32_t i = 0; i < 8; i++) {
-            const uint32_t b = i / 4, key = min(k_begin + 32 * step + 16 * b + 4 * g + i % 4, k_end - 1);
-            if (pg[b] != KV_NO_PAGE) { // uniform
-                const uint8_t* row = vbase + kv_row(a.c, pg[b], kv, key, DH) * ES;
-#pragma unroll
-                for (uint32_t c = c0; c < c1; c++) vreg[c][i] = *(const u32x4*)(row + (c * 16 + m) * 16);
-            } else {
-#pragma unroll
-                for (uint32_t c = c0; c < c1; c++) vreg[c][i] = zero;
-            }
-        }
-    };
-    uint32_t pg[2], pg_next[2];
-    pages(wave, pg);
-    if (wave < n_step) {
-        fetch_k(wave, 0, pg);
-        fetch_k(wave, 1, pg);
-    }
     for (uint32_t step = wave; step < n_step; step += 4) {
-        const uint32_t key0 = k_begin + 32 * step;
+        const uint32_t key0 = k_begin + SK * step;
         pages(step + 4, pg_next);
         // scores
-        float4v s[RT][2];
+        float4v s[RT][2 * SUB];
 #pragma unroll
-        for (uint32_t b = 0; b < 2; b++) {
+        for (uint32_t b = 0; b < 2 * SUB; b++) {
 #pragma unroll
             for (uint32_t rt = 0; rt < RT; rt++) s[rt][b] = float4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (uint32_t ks = 0; ks < KS; ks++) {
+                const u32x4* kr = kreg[b / 2][b % 2][ks];
                 if constexpr (F32) {
                     float x[8];
 #pragma unroll
-                    for (uint32_t i = 0; i < 8; i++) x[i] = u2f(kreg[b][ks][i / 4][i % 4]);
+                    for (uint32_t i = 0; i < 8; i++) x[i] = u2f(kr[i / 4][i % 4]);
                     const Bf3 k3 = split3(x);
 #pragma unroll
                     for (uint32_t rt = 0; rt < RT; rt++) {
@@ -188,7 +210,7 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(RunsCall a)
                         s[rt][b] = mfma16x32(k3.p[0], qq[0], s[rt][b]);
                     }
                 } else {
-                    const half8 kh = __builtin_bit_cast(half8, kreg[b][ks][0]);
+                    const half8 kh = __builtin_bit_cast(half8, u32x4(kr[0]));
 #pragma unroll
                     for (uint32_t rt = 0; rt < RT; rt++) {
                         s[rt][b] = mfma16x32(kh, __builtin_bit_cast(half8, u32x4(q_op[((RT + rt) * KS + ks) * 64 + lane])), s[rt][b]);
@@ -197,45 +219,61 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(RunsCall a)
                 }
                 if (ks % 2) __builtin_amdgcn_sched_barrier(0); // the Q operand's reads stay near their use: registers
             }
-            if (b == 0) fetch_v(step, 0, CA, pg);
-            else if (CA < NC) fetch_v(step, CA, NC, pg);
+            if (HALVES) {
+                if (b == 0) fetch_v(step, 0, 0, CA, pg);
+                else fetch_v(step, 0, CA, NC, pg);
+            } else fetch_k(step + 4, b, pg_next);
             __builtin_amdgcn_sched_barrier(0);
         }
         // softmax: this lane's row 16 rt + m, keys 16 b + 4 g + r
-        const bool whole = key0 + 32 <= k_end && pg[0] != KV_NO_PAGE && pg[1] != KV_NO_PAGE && key0 + 32 <= u.pos + (TREE ? 0u : 1u); // uniform
-        float p[RT][8];
+        bool whole = key0 + SK <= k_end && key0 + SK <= u.pos + (TREE ? 0u : 1u); // uniform
+#pragma unroll
+        for (uint32_t b = 0; b < 2 * SUB; b++) whole = whole && pg[b] != KV_NO_PAGE;
         uint32_t seen[RT]; // bit 4 b + r: the row sees that key
+        Bf3 p3[RT][SUB];
+        Half2 p2[RT][SUB];
 #pragma unroll
         for (uint32_t rt = 0; rt < RT; rt++) {
             const float cf = qs * q_exp[rt];
-            seen[rt] = 0xFFu;
-            if (!whole) {
+#pragma unroll
+            for (uint32_t b = 0; b < 2 * SUB; b++) s[rt][b] *= cf;
+            seen[rt] = 0xFFFFu;
+            if (!whole) { // uniform
                 const uint32_t f = 16 * rt + m, node = min(f, nr - 1) / a.G;
                 seen[rt] = 0;
 #pragma unroll
-                for (uint32_t i = 0; i < 8; i++) {
-                    const uint32_t key = key0 + 16 * (i / 4) + 4 * g + i % 4;
-                    bool v = key < k_end && pg[i / 4] != KV_NO_PAGE && f < nr;
-                    if (v && key >= u.pos) v = TREE ? (s_kin[node][(key - u.pos) >> 5] >> ((key - u.pos) & 31u)) & 1u : key - u.pos <= node;
-                    seen[rt] |= (v ? 1u : 0u) << i;
+                for (uint32_t b = 0; b < 2 * SUB; b++) { // four neighbouring keys at a time
+                    const uint32_t key = key0 + 16 * b + 4 * g;
+                    const uint32_t stop = pg[b] == KV_NO_PAGE || f >= nr ? 0u : TREE ? k_end : min(k_end, u.pos + node + 1);
+                    uint32_t four = (1u << (stop > key ? min(stop - key, 4u) : 0u)) - 1u;
+                    if (drafts) four &= tree_four(s_kin[node], (int32_t)(key - u.pos));
+                    seen[rt] |= four << (4 * b);
+#pragma unroll
+                    for (uint32_t r = 0; r < 4; r++) s[rt][b][r] = (four >> r) & 1u ? s[rt][b][r] : -INFINITY;
                 }
             }
             float mx = AR_FLOOR;
 #pragma unroll
-            for (uint32_t i = 0; i < 8; i++) {
-                p[rt][i] = s[rt][i / 4][i % 4] * cf;
-                if (whole) mx = fmaxf(mx, p[rt][i]);
-                else mx = fmaxf(mx, (seen[rt] >> i) & 1u ? p[rt][i] : AR_FLOOR);
-            }
+            for (uint32_t i = 0; i < 8 * SUB; i++) mx = fmaxf(mx, s[rt][i / 4][i % 4]);
             const float m_new = fmaxf(m_run[rt], xor_lanes_max(mx));
             const float corr = __builtin_amdgcn_exp2f(m_run[rt] - m_new);
             m_run[rt] = m_new;
             float sum = 0.f;
 #pragma unroll
-            for (uint32_t i = 0; i < 8; i++) {
-                const float w = __builtin_amdgcn_exp2f(p[rt][i] - m_new);
-                p[rt][i] = whole || ((seen[rt] >> i) & 1u) ? w : 0.f;
-                sum += p[rt][i];
+            for (uint32_t sb = 0; sb < SUB; sb++) {
+                float p[8];
+#pragma unroll
+                for (uint32_t i = 0; i < 8; i++) {
+                    p[i] = __builtin_amdgcn_exp2f(s[rt][2 * sb + i / 4][i % 4] - m_new);
+                    sum += p[i];
+                }
+                // weights of a half cache up to 2^14, so that the lo halves of small ones stay normal; undone at the end
+                if constexpr (F32) p3[rt][sb] = split3(p);
+                else {
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; i++) p[i] *= 16384.f;
+                    p2[rt][sb] = split2(p);
+                }
             }
             l_run[rt] = l_run[rt] * corr + sum; // of this lane's keys; the lane groups are added at the end
             if (__builtin_amdgcn_ballot_w64(corr != 1.f)) { // uniform
@@ -245,8 +283,8 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(RunsCall a)
         }
         // Where not every row sees every key, values that are not finite are taken out of the product (a weight of zero would not
         // keep them out) and added to the rows that do see them.
-        uint32_t odd = 0; // bit i: the lane's key i of 8 holds such a value
-        auto clean = [&](uint32_t c0, uint32_t c1) {
+        uint32_t odd = 0; // bit 8 sb + i: the lane's key i of 8 holds such a value
+        auto clean = [&](uint32_t sb, uint32_t c0, uint32_t c1) {
 #pragma unroll
             for (uint32_t i = 0; i < 8; i++) {
                 bool bad = false;
@@ -254,35 +292,22 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(RunsCall a)
                 for (uint32_t c = c0; c < c1; c++)
 #pragma unroll
                     for (uint32_t w = 0; w < 4; w++) {
-                        const uint32_t x = vreg[c][i][w];
+                        const uint32_t x = vreg[sb][c][i][w];
                         if (F32) {
                             const bool b1 = (x & 0x7F800000u) == 0x7F800000u;
                             bad = bad || b1;
-                            vreg[c][i][w] = b1 ? 0u : x;
+                            vreg[sb][c][i][w] = b1 ? 0u : x;
                         } else {
                             const bool b0 = (x & 0x7C00u) == 0x7C00u, b1 = (x & 0x7C000000u) == 0x7C000000u;
                             bad = bad || b0 || b1;
-                            vreg[c][i][w] = (b0 ? 0u : x & 0xFFFFu) | (b1 ? 0u : x & 0xFFFF0000u);
+                            vreg[sb][c][i][w] = (b0 ? 0u : x & 0xFFFFu) | (b1 ? 0u : x & 0xFFFF0000u);
                         }
                     }
                 const uint64_t who = __builtin_amdgcn_ballot_w64(bad);
-                odd |= ((who >> (16 * g)) & 0xFFFFu ? 1u : 0u) << i;
+                odd |= ((who >> (16 * g)) & 0xFFFFu ? 1u : 0u) << (8 * sb + i);
             }
         };
-        // weights of a half cache up to 2^14, so that the lo halves of small ones stay normal; undone at the end
-        Bf3 p3[RT];
-        Half2 p2[RT];
-#pragma unroll
-        for (uint32_t rt = 0; rt < RT; rt++) {
-            if constexpr (F32) p3[rt] = split3(p[rt]);
-            else {
-                float x[8];
-#pragma unroll
-                for (uint32_t i = 0; i < 8; i++) x[i] = p[rt][i] * 16384.f;
-                p2[rt] = split2(x);
-            }
-        }
-        auto values = [&](uint32_t c0, uint32_t c1) {
+        auto values = [&](uint32_t sb, uint32_t c0, uint32_t c1) {
 #pragma unroll
             for (uint32_t c = c0; c < c1; c++)
 #pragma unroll
@@ -290,52 +315,60 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(RunsCall a)
                     if constexpr (F32) {
                         float x[8];
 #pragma unroll
-                        for (uint32_t i = 0; i < 8; i++) x[i] = u2f(vreg[c][i][e]);
+                        for (uint32_t i = 0; i < 8; i++) x[i] = u2f(vreg[sb][c][i][e]);
                         const Bf3 v3 = split3(x);
 #pragma unroll
                         for (uint32_t rt = 0; rt < RT; rt++) {
                             float4v& acc = o[rt][c * E + e];
-                            acc = mfma16x32(v3.p[2], p3[rt].p[0], acc);
-                            acc = mfma16x32(v3.p[0], p3[rt].p[2], acc);
-                            acc = mfma16x32(v3.p[1], p3[rt].p[1], acc);
-                            acc = mfma16x32(v3.p[1], p3[rt].p[0], acc);
-                            acc = mfma16x32(v3.p[0], p3[rt].p[1], acc);
-                            acc = mfma16x32(v3.p[0], p3[rt].p[0], acc);
+                            acc = mfma16x32(v3.p[2], p3[rt][sb].p[0], acc);
+                            acc = mfma16x32(v3.p[0], p3[rt][sb].p[2], acc);
+                            acc = mfma16x32(v3.p[1], p3[rt][sb].p[1], acc);
+                            acc = mfma16x32(v3.p[1], p3[rt][sb].p[0], acc);
+                            acc = mfma16x32(v3.p[0], p3[rt][sb].p[1], acc);
+                            acc = mfma16x32(v3.p[0], p3[rt][sb].p[0], acc);
                         }
                     } else {
                         u32x4 w;
 #pragma unroll
                         for (uint32_t i = 0; i < 4; i++) // half e of keys 2 i, 2 i + 1
-                            w[i] = __builtin_amdgcn_perm(vreg[c][2 * i + 1][e / 2], vreg[c][2 * i][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+                            w[i] = __builtin_amdgcn_perm(vreg[sb][c][2 * i + 1][e / 2], vreg[sb][c][2 * i][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
                         const half8 vh = __builtin_bit_cast(half8, w);
 #pragma unroll
                         for (uint32_t rt = 0; rt < RT; rt++) {
                             float4v& acc = o[rt][c * E + e];
-                            acc = mfma16x32(vh, p2[rt].lo, acc);
-                            acc = mfma16x32(vh, p2[rt].hi, acc);
+                            acc = mfma16x32(vh, p2[rt][sb].lo, acc);
+                            acc = mfma16x32(vh, p2[rt][sb].hi, acc);
                         }
                     }
                 }
         };
-        if (!whole) clean(0, CA);
-        values(0, CA);
-        __builtin_amdgcn_sched_barrier(0);
-        fetch_k(step + 4, 0, pg_next); // behind the last step: zeros, no load (and no register held for what is not read again)
-        if (CA < NC) {
-            if (!whole) clean(CA, NC);
-            values(CA, NC);
+        if (HALVES) {
+            if (!whole) clean(0, 0, CA);
+            values(0, 0, CA);
             __builtin_amdgcn_sched_barrier(0);
+            fetch_k(step + 4, 0, pg_next);
+            if (!whole) clean(0, CA, NC);
+            values(0, CA, NC);
+            __builtin_amdgcn_sched_barrier(0);
+            fetch_k(step + 4, 1, pg_next);
+        } else {
+#pragma unroll
+            for (uint32_t sb = 0; sb < SUB; sb++) {
+                if (!whole) clean(sb, 0, NC);
+                values(sb, 0, NC);
+                __builtin_amdgcn_sched_barrier(0);
+                fetch_v(step + 4, sb, 0, NC, pg_next);
+            }
         }
-        fetch_k(step + 4, 1, pg_next);
         __builtin_amdgcn_sched_barrier(0);
         if (__builtin_amdgcn_ballot_w64(odd != 0)) { // rare: uniform
-            for (uint32_t kk = 0; kk < 32; kk++) {
-                const uint32_t kg = kk % 16 / 4, i = kk / 16 * 4 + kk % 4; // lane group and place of key kk
+            for (uint32_t kk = 0; kk < SK; kk++) {
+                const uint32_t kg = kk % 16 / 4, i = kk / 16 * 4 + kk % 4; // lane group and place (bit) of key kk
                 const uint32_t flags = (uint32_t)__shfl((int)odd, (int)(16 * kg));
                 if (!((flags >> i) & 1u)) continue; // uniform
-                const uint32_t key = key0 + 16 * (kk / 16) + kk % 16;
+                const uint32_t key = key0 + kk;
                 if (key >= k_end) continue; // uniform (rows behind the range repeat its last one)
-                const uint8_t* row = vbase + kv_row(a.c, pg[kk / 16], kv, key, DH) * ES;
+                const uint8_t* row = vbase + kv_row(a.c, kv_page(a.c, u.seq, key), kv, key, DH) * ES;
 #pragma unroll
                 for (uint32_t rt = 0; rt < RT; rt++) {
                     const bool sees = ((uint32_t)__shfl((int)seen[rt], (int)(16 * kg + m)) >> i) & 1u;
@@ -354,8 +387,8 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(RunsCall a)
                 }
             }
         }
-        pg[0] = pg_next[0];
-        pg[1] = pg_next[1];
+#pragma unroll
+        for (uint32_t b = 0; b < 2 * SUB; b++) pg[b] = pg_next[b];
     }
 
     // the four waves' partial results: 2, 3 into 0, 1, then 1 into 0

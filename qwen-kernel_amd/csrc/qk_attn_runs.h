@@ -111,11 +111,15 @@ __device__ __forceinline__ int top_exponent(float m)
 __device__ __forceinline__ float pow2i(int e) { return u2f((uint32_t)(e + 127) << 23); }
 
 // Ancestors of the nodes node0 .. node0 + n - 1 of a run as bits, kin[n][QKK_TREE_MAX / 32] in LDS; s_up: the run's parents
-// (QKK_TREE_MAX entries).  The whole workgroup calls it (two barriers).
-__device__ __forceinline__ void tree_bits(const int32_t* __restrict__ parent, const Run& u, uint32_t node0, uint32_t n, int32_t* s_up,
-                                          uint32_t (*kin)[QKK_TREE_MAX / 32])
+// (QKK_TREE_MAX entries), thread i brings node i's (requested early: tree_parent).  The whole workgroup, at least QKK_TREE_MAX
+// threads, calls it (two barriers).
+__device__ __forceinline__ int32_t tree_parent(const int32_t* __restrict__ parent, const Run& u)
 {
-    for (uint32_t i = threadIdx.x; i < u.n; i += blockDim.x) s_up[i] = parent[u.r0 + i];
+    return threadIdx.x < u.n ? parent[u.r0 + threadIdx.x] : -1;
+}
+__device__ __forceinline__ void tree_bits(int32_t up_of, uint32_t node0, uint32_t n, int32_t* s_up, uint32_t (*kin)[QKK_TREE_MAX / 32])
+{
+    if (threadIdx.x < QKK_TREE_MAX) s_up[threadIdx.x] = up_of;
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
         uint32_t w[QKK_TREE_MAX / 32] = {};
@@ -139,6 +143,23 @@ __device__ __forceinline__ void tree_bits(const int32_t* __restrict__ parent, co
 // do not fit the registers)
 constexpr uint32_t few_rows(uint32_t dh) { return dh == 128 ? 32 : 16; }
 
+// Which of four neighbouring keys, the first `rel` rows behind the tree's first row (negative: in front of the tree), a node sees.
+__device__ __forceinline__ uint32_t tree_four(const uint32_t* kin, int32_t rel)
+{
+    constexpr uint32_t W = QKK_TREE_MAX / 32;
+    const uint32_t before = (uint32_t)min(max(-rel, 0), 4), at = (uint32_t)max(rel, 0), w = min(at >> 5, W - 1); // no branches
+    const uint32_t lo = kin[w], hi = kin[min(w + 1, W - 1)];
+    const uint64_t both = ((uint64_t)(w + 1 < W ? hi : 0u) << 32) | lo;
+    const uint32_t bits = at < QKK_TREE_MAX ? (uint32_t)(both >> (at & 31u)) : 0u;
+    return ((bits << before) | ((1u << before) - 1u)) & 15u;
+}
+
+// query rows (positions x heads of a group) per workgroup of the kernel for many rows, and its blocks of them: a run's blocks begin
+// at its own first row, so every run may have one that is not full
+constexpr uint32_t AR_TILE_ROWS = 128;
+inline uint32_t tile_blocks(uint32_t n_rows, uint32_t n_run, uint32_t G) { return (uint32_t)((uint64_t)n_rows * G / AR_TILE_ROWS) + n_run; }
+
 void launch_attn_few(const RunsCall& call, int type, uint32_t dh, bool tree, hipStream_t st);
+void launch_attn_tile(const RunsCall& call, int type, uint32_t dh, bool tree, hipStream_t st);
 
 } // namespace qk

@@ -8,83 +8,6 @@
 
 namespace qk {
 
-constexpr uint32_t AR_TILE = 64;  // cache rows scored per pass
-
-// grid (rows, hQ), 256 threads: one row's head, tile after tile of the cache with the running maximum and sum.
-template <int DH, typename T, bool TREE>
-__global__ __launch_bounds__(256) void attn_runs_plain_kernel(KvView c, RunsView R, const int32_t* __restrict__ parent,
-                                                              const float* __restrict__ q, const float* __restrict__ qfull,
-                                                              float* __restrict__ att, uint32_t hQ)
-{
-    __shared__ float s_q[DH], s_p[AR_TILE], s_acc[256], s_m, s_l, s_corr;
-    __shared__ uint32_t s_kin[QKK_TREE_MAX / 32];
-    const uint32_t row = blockIdx.x, h = blockIdx.y, t = threadIdx.x, lane = t & 63u, wave = t >> 6;
-    const uint32_t ri = wave_last_le(R.n_run, row, [&](uint32_t i) { return (int64_t)R.start[i]; });
-    if (ri >= R.n_run) return; // the whole workgroup
-    const Run u = run_at(c, R, ri);
-    if (!u.ok || row - u.r0 >= u.n) return; // the whole workgroup
-    const uint32_t node = row - u.r0, kv = h / (hQ / c.n_kv);
-    for (uint32_t d = t; d < DH; d += 256) s_q[d] = q[((size_t)row * hQ + h) * DH + d];
-    if (t < QKK_TREE_MAX / 32) s_kin[t] = 0;
-    if (t == 0) { s_m = AR_FLOOR; s_l = 0.f; }
-    __syncthreads();
-    if (TREE && t == 0)
-        for (int32_t a = (int32_t)node;;) {
-            s_kin[a >> 5] |= 1u << (a & 31);
-            const int32_t up = parent[u.r0 + a];
-            if (up < 0 || up >= a) break;
-            a = up;
-        }
-    __syncthreads();
-    const float qs = 1.f / sqrtf((float)DH);
-    const T* K = (const T*)c.k;
-    const T* V = (const T*)c.v;
-    constexpr uint32_t PARTS = 256 / DH; // threads that share a dim
-    float acc = 0.f;
-    const uint32_t end = min(u.pos + node + 1, c.cap);
-    for (uint32_t p0 = 0; p0 < end; p0 += AR_TILE) {
-        // scores: 4 lanes per key
-        const uint32_t key = p0 + (t >> 2);
-        float s = 0.f;
-        bool sees = key < end && (!TREE || key < u.pos || ((s_kin[(key - u.pos) >> 5] >> ((key - u.pos) & 31)) & 1u));
-        const uint32_t page = sees ? kv_page(c, u.seq, key) : KV_NO_PAGE;
-        sees = page != KV_NO_PAGE;
-        if (sees) {
-            const T* row_k = K + kv_row(c, page, kv, key, DH);
-            for (uint32_t d = t & 3u; d < DH; d += 4) s += s_q[d] * (float)row_k[d];
-        }
-        s = group_sum<4>(s);
-        if ((t & 3u) == 0) s_p[t >> 2] = sees ? s * qs : -INFINITY;
-        __syncthreads();
-        if (wave == 0) {
-            const float v = s_p[lane];
-            const float m = fmaxf(s_m, wave_max(v));
-            const float e = v == -INFINITY ? 0.f : expf(v - m), sum = wave_sum(e);
-            s_p[lane] = v == -INFINITY ? -1.f : e; // negative: not seen
-            if (lane == 0) {
-                s_corr = expf(s_m - m);
-                s_l = s_l * s_corr + sum;
-                s_m = m;
-            }
-        }
-        __syncthreads();
-        acc *= s_corr;
-        const uint32_t d = t % DH;
-        for (uint32_t i = t / DH; i < AR_TILE && p0 + i < end; i += PARTS)
-            if (s_p[i] >= 0.f || s_p[i] != s_p[i]) acc += s_p[i] * (float)V[kv_row(c, kv_page(c, u.seq, p0 + i), kv, p0 + i, DH) + d];
-        __syncthreads(); // the next tile overwrites the scores
-    }
-    s_acc[t] = acc;
-    __syncthreads();
-    if (t < DH) {
-        float o = 0.f;
-        for (uint32_t i = 0; i < PARTS; i++) o += s_acc[t + i * DH];
-        o = s_l == 0.f ? 0.f : o / s_l;
-        if (qfull) o *= 1.f / (1.f + expf(-qfull[((size_t)row * hQ + h) * 2 * DH + DH + t]));
-        att[((size_t)row * hQ + h) * DH + t] = o;
-    }
-}
-
 // One wave per (row, head): folds the ranges in range order and applies the gate.  Ranges behind the row's own position hold
 // nothing for it.
 template <int DH>
@@ -146,12 +69,19 @@ static Plan plan_of(const qkk_kv_cache* C, const qkk_kv_runs* R, uint32_t hQ)
     const uint64_t cap = (uint64_t)C->seq_pages * C->page_rows;
     Plan p;
     p.few = (uint64_t)max_run * G <= few_rows(C->dh);
-    if (!p.few) return Plan{false, 1, (uint32_t)cap};
-    // ranges of 128 keys (a step per wave) while about a thousand workgroups cover the whole cache with them, longer ones beyond;
-    // at most 64 (the join's lanes)
-    const uint64_t units = (uint64_t)R->n_run * C->n_kv;
-    const uint64_t want = std::max((cap * units + 1023) / 1024, (cap + 63) / 64);
-    p.chunk = (uint32_t)std::max<uint64_t>(128, (want + 127) / 128 * 128);
+    if (!p.few) {
+        // one range where the blocks of rows fill the chip (one workgroup per CU), else about two workgroups per CU
+        const uint64_t groups = std::max<uint64_t>(((uint64_t)R->n_rows * G + AR_TILE_ROWS - 1) / AR_TILE_ROWS, R->n_run) * C->n_kv;
+        const uint64_t ranges = groups >= 256 ? 1 : std::min<uint64_t>(64, (512 + groups - 1) / groups);
+        p.chunk = (uint32_t)std::max<uint64_t>(128, ((cap + ranges - 1) / ranges + 127) / 128 * 128);
+        p.n_split = (uint32_t)((cap + p.chunk - 1) / p.chunk);
+        return p;
+    }
+    // ranges of one step per wave (128 keys, 256 for halves with dh 128) while about two thousand workgroups cover the whole cache
+    // with them, longer ones beyond; at most 64 (the join's lanes)
+    const uint64_t units = (uint64_t)R->n_run * C->n_kv, step = C->type == QKK_F16 && C->dh == 128 ? 256 : 128;
+    const uint64_t want = std::max((cap * units + 2047) / 2048, (cap + 63) / 64);
+    p.chunk = (uint32_t)std::max<uint64_t>(step, (want + step - 1) / step * step);
     p.n_split = (uint32_t)((cap + p.chunk - 1) / p.chunk);
     return p;
 }
@@ -174,9 +104,9 @@ static int attn_runs(const char* who, const qkk_kv_cache* C, uint32_t layer, con
     if (int rc = require_device()) return rc;
     if (!runs.n_rows || !runs.n_run) return QKK_OK;
     const Plan plan = plan_of(C, R, hQ);
-    if ((uint64_t)runs.n_run * c.n_kv * plan.n_split > (1u << 30) || (uint64_t)runs.n_rows * hQ > (1u << 30))
+    if ((uint64_t)(tile_blocks(runs.n_rows, runs.n_run, hQ / c.n_kv)) * c.n_kv * plan.n_split > (1u << 30) || (uint64_t)runs.n_rows * hQ > (1u << 30))
         return fail(QKK_ESHAPE, "%s: rows x heads or runs x heads too large", who);
-    if (plan.few) {
+    {
         RunsCall a;
         a.c = c;
         a.R = runs;
@@ -190,27 +120,14 @@ static int attn_runs(const char* who, const qkk_kv_cache* C, uint32_t layer, con
         a.G = hQ / c.n_kv;
         a.n_split = plan.n_split;
         a.chunk = plan.chunk;
-        launch_attn_few(a, C->type, C->dh, tree, as_stream(stream));
+        if (plan.few) launch_attn_few(a, C->type, C->dh, tree, as_stream(stream));
+        else launch_attn_tile(a, C->type, C->dh, tree, as_stream(stream));
         if (plan.n_split > 1) {
             const dim3 jobs((uint32_t)(((uint64_t)runs.n_rows * hQ + 3) / 4));
             if (C->dh == 256) hipLaunchKernelGGL(attn_join_kernel<256>, jobs, dim3(256), 0, as_stream(stream), a);
             else hipLaunchKernelGGL(attn_join_kernel<128>, jobs, dim3(256), 0, as_stream(stream), a);
         }
-        return check_launch(who);
     }
-    const dim3 grid(runs.n_rows, hQ), block(256);
-#define QK_RUNS(DH, T, TREE)                                                                                                             \
-    hipLaunchKernelGGL((attn_runs_plain_kernel<DH, T, TREE>), grid, block, 0, as_stream(stream), c, runs, parent, qhat, qfull, att, hQ)
-#define QK_RUNS2(DH, T) do { if (tree) QK_RUNS(DH, T, true); else QK_RUNS(DH, T, false); } while (0)
-    if (C->dh == 256) {
-        if (C->type == QKK_F32) QK_RUNS2(256, float);
-        else QK_RUNS2(256, _Float16);
-    } else {
-        if (C->type == QKK_F32) QK_RUNS2(128, float);
-        else QK_RUNS2(128, _Float16);
-    }
-#undef QK_RUNS2
-#undef QK_RUNS
     return check_launch(who);
 }
 

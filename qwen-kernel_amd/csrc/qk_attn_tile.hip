@@ -1,0 +1,517 @@
+// qk_attn_tile.hip -- attention of runs with MANY query rows (prompts, wide trees) over the paged cache: tiles of 128 query
+// rows (positions x heads of one KV head's group), keys staged through LDS as matrix-core operands.
+//
+// A workgroup takes 128 rows of one run and one KV head, each of its waves 16 (dh 256) or 32 (dh 128) of them from end to end, its
+// Q operand and its accumulators in registers: two waves per SIMD, so one's softmax runs beside another's products.  A
+// tile of 32 (fp32) or 64 (half) keys goes from the cache to registers while the tile before it is worked on -- half of the waves
+// load K, the others V -- and from there to the other one of two LDS buffers:
+//   K    as it lies, [key][dim] halves (row pitch + 16 bytes: 16 lanes fall on 16 different bank groups);
+//   V^T  [dim][key]: a thread holds 8 keys x 4 (fp32) or 8 (half) dims, in the order of keys that the weights P have in the
+//        registers of the first product, and writes 16 bytes per dim.
+// One barrier per tile.  Matrix work per key and row: 4 dh operations times the products of split operands.
+//   F16 cache   K and V are operands as they are, Q and P are hi + lo halves: two products.
+//   F32 cache   every row of K and V is divided by the power of two that brings its largest value into [1, 2) and split
+//               into hi + lo halves, three products (lo . lo is below 2^-22 of its term).  The powers of two go back in where they
+//               cost nothing: a key's into the factor of its scores, a value row's into the exponent of its weight -- P V = (P 2^e)
+//               (V 2^-e), so the running maximum is kept over score + e -- and out of the sum again.  So fp32's range holds,
+//               row by row, with half the matrix work of three bf16 pieces.
+// Weights are kept around 2^6 rather than 1, which keeps the lo halves of small ones normal; the sum has the same factor.
+#include "qk_attn_runs.h"
+
+namespace qk {
+
+typedef u32x4 __attribute__((may_alias)) lds_u32x4;
+typedef u32x2 __attribute__((may_alias)) lds_u32x2;
+typedef f32x4 __attribute__((may_alias)) lds_f32x4;
+
+constexpr uint32_t TL_M = AR_TILE_ROWS;
+// The running maximum is moved only when a score passes it by more than 2^TL_SLACK: weights stay below 2^(TL_UP + TL_SLACK), inside a
+// half's range, and most tiles need neither an exchange between lanes nor a rescaling of the accumulators.
+constexpr float TL_UP = 6.f, TL_SLACK = 8.f;
+constexpr int TL_VMIN = -90; // smallest exponent of a value row: a row of zeros keeps its weight in the sum
+
+template <int DH, bool F32>
+struct TileGeom {
+    static constexpr uint32_t ES = F32 ? 4 : 2, NH = F32 ? 2 : 1;
+    static constexpr uint32_t WAVES = DH / 32;                     // dh 128: 4 waves of 32 rows, two workgroups per CU; 256: 8 waves of 16 rows, one
+    static constexpr uint32_t RT = TL_M / WAVES / 16;              // blocks of 16 rows per wave
+    static constexpr uint32_t LPR = DH * ES / 16;                  // 16-byte pieces of a row = lanes that load one
+    static constexpr uint32_t NB = F32 ? 1 : 2, BN = 32 * NB;      // steps of 32 keys per tile
+    static constexpr uint32_t KP = DH * 2 + 16, VP = NB * 64 + 16; // row pitches, bytes
+    static constexpr uint32_t KB = BN * KP, VB = DH * VP;          // one copy of K, of V^T
+    static constexpr uint32_t EXP = F32 ? 3 * BN * 4 : 0;          // per key: factor of the score, exponent and factor of the value row
+    static constexpr uint32_t BUF = NH * (KB + VB) + EXP + 64;     // + flags [4 NB]
+    // half of the waves stage K, the others V: eight pieces per thread
+    static_assert(NB * LPR * 4 == WAVES * 32, "staging");
+};
+
+// Maxima of eight rows' magnitudes (as integers, so NaN counts as the largest) over the LPR lanes that hold a row: after the
+// first two steps a lane holds two rows' values (row 4 k + lane % 4, k = 0, 1), which the other steps reduce over the lanes
+// with the same lane % 4.  Returns both.
+template <uint32_t LPR>
+__device__ __forceinline__ void rows_max(const uint32_t* v, uint32_t* out)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t a[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const uint32_t keep = lane & 1u ? v[2 * k + 1] : v[2 * k], give = lane & 1u ? v[2 * k] : v[2 * k + 1];
+        a[k] = max(keep, (uint32_t)dpp_i<DPP_XOR1>((int)give));
+    }
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const uint32_t keep = lane & 2u ? a[2 * k + 1] : a[2 * k], give = lane & 2u ? a[2 * k] : a[2 * k + 1];
+        uint32_t b = max(keep, (uint32_t)dpp_i<DPP_XOR2>((int)give));
+        b = max(b, (uint32_t)dpp_i<0x124>((int)b)); // row_ror 4
+        b = max(b, (uint32_t)dpp_i<0x128>((int)b)); // row_ror 8
+        if (LPR > 16) b = max(b, (uint32_t)__shfl_xor((int)b, 16));
+        if (LPR > 32) b = max(b, (uint32_t)__shfl_xor((int)b, 32));
+        out[k] = b;
+    }
+}
+// value of lane q of the own group of four lanes
+template <int Q>
+__device__ __forceinline__ float quad_lane(float v)
+{
+    return dpp_f<Q * 0x55>(v);
+}
+__device__ __forceinline__ void quad_spread(const float* two, float* eight) // [row 4 k + q] from lane q of the quad
+{
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        eight[4 * k] = quad_lane<0>(two[k]);
+        eight[4 * k + 1] = quad_lane<1>(two[k]);
+        eight[4 * k + 2] = quad_lane<2>(two[k]);
+        eight[4 * k + 3] = quad_lane<3>(two[k]);
+    }
+}
+
+template <int DH, bool F32, bool TREE>
+__global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_kernel(RunsCall a)
+{
+    using T = TileGeom<DH, F32>;
+    constexpr uint32_t KS = DH / 32, NT = DH / 16, LPR = T::LPR, NB = T::NB, BN = T::BN, E = F32 ? 4 : 8, NC = LPR / 16, RT = T::RT, WR = 16 * RT;
+    QK_DYN_LDS(uint8_t, s_dyn);
+    __shared__ int32_t s_up[TREE ? QKK_TREE_MAX : 1];
+    __shared__ uint32_t s_kin[TREE ? TL_M : 1][QKK_TREE_MAX / 32];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, m = lane & 15u, g = lane >> 4;
+
+    // workgroup -> KV head, block of rows (the last, longest ones first), range of keys.  Workgroups go to the eight dies in turn: with
+    // the range varying slowest every die gets its share of the first ranges, which every block has.  A run's blocks begin at its
+    // own first row; run i's first block has the number floor(start G / 128) + i, which leaves every run room for its
+    // last, part-filled one.
+    const uint32_t n_blocks = gridDim.x / a.c.n_kv / a.n_split;
+    const uint32_t kv = blockIdx.x % a.c.n_kv, blk = n_blocks - 1 - blockIdx.x / a.c.n_kv % n_blocks, split = blockIdx.x / a.c.n_kv / n_blocks;
+    auto first_of = [&](uint32_t i) { return (int64_t)((uint64_t)max(a.R.start[i], 0) * a.G / TL_M) + i; };
+    const uint32_t run = wave_last_le(a.R.n_run, blk, first_of);
+    if (run >= a.R.n_run) return; // the whole workgroup
+    const Run u = run_at(a.c, a.R, run);
+    const uint32_t f0 = (blk - (uint32_t)first_of(run)) * TL_M, rows_all = u.n * a.G;
+    if (!u.ok || f0 >= rows_all) return; // the whole workgroup
+    const uint32_t nr = min(TL_M, rows_all - f0);
+    const uint32_t last = (f0 + nr - 1) / a.G; // the block's last position in the run
+    const uint32_t end = min(u.pos + last + 1, a.c.cap), k_begin = split * a.chunk;
+    if (k_begin >= end) return; // the whole workgroup
+    const uint32_t k_end = min(end, k_begin + a.chunk), n_tile = (k_end - k_begin + BN - 1) / BN;
+    const uint32_t node0 = f0 / a.G;
+    if (TREE && k_end > u.pos) tree_bits(tree_parent(a.parent, u), node0, last - node0 + 1, s_up, s_kin);
+
+    // Q: this wave's rows f0 + WR wave + 16 rt + m, dims 32 ks + 8 g .. + 7, divided by the row's power of two
+    half8 qh[RT][KS], ql[RT][KS];
+    float q_fac[RT];
+    const uint32_t wr = WR * wave; // the wave's first row in the block
+    const bool has = wr < nr;      // uniform: a wave without rows only stages tiles
+#pragma unroll
+    for (uint32_t rt = 0; rt < RT; rt++) {
+        const uint32_t f = wr + 16 * rt + m, ff = f0 + min(f, nr - 1);
+        const f32x4* row = (const f32x4*)(a.q + ((size_t)(u.r0 + ff / a.G) * a.hQ + kv * a.G + ff % a.G) * DH);
+        f32x4 x[KS][2];
+        float mx = 0.f;
+#pragma unroll
+        for (uint32_t ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (uint32_t i = 0; i < 2; i++) {
+                x[ks][i] = row[8 * ks + 2 * g + i];
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) mx = fmaxf(mx, fabsf(x[ks][i][j]));
+            }
+        const int e = top_exponent(xor_lanes_max(mx));
+        const float scale = pow2i(-e);
+        q_fac[rt] = pow2i(e) * (AR_LOG2E / sqrtf((float)DH));
+#pragma unroll
+        for (uint32_t ks = 0; ks < KS; ks++) {
+            float y[8];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) y[j] = x[ks][j / 4][j % 4] * scale;
+            const Half2 sp = split2(y);
+            qh[rt][ks] = sp.hi;
+            ql[rt][ks] = sp.lo;
+        }
+    }
+    float4v o[RT][NT];
+    float m_run[RT], l_run[RT];
+#pragma unroll
+    for (uint32_t rt = 0; rt < RT; rt++) {
+        m_run[rt] = AR_FLOOR;
+        l_run[rt] = 0.f;
+#pragma unroll
+        for (uint32_t t = 0; t < NT; t++) o[rt][t] = float4v{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // this lane's rows' positions behind node0 (below 128), 255 for a row that is not there: a byte for each block, so one register
+    uint32_t nodes = 0;
+#pragma unroll
+    for (uint32_t rt = 0; rt < RT; rt++) nodes |= (wr + 16 * rt + m < nr ? (f0 + wr + 16 * rt + m) / a.G - node0 : 0xFFu) << (8 * rt);
+    const uint32_t first_node = (f0 + min(wr, nr - 1)) / a.G, last_node = (f0 + min(wr + WR, nr) - 1) / a.G;
+
+    // Staging: the first half of the waves takes V, the second K.  A thread: (piece of a row, lane group sg of the second
+    // product, step of 32 keys st), its eight keys of that step 4 sg + i and 16 + 4 sg + i.
+    const bool is_v = wave < T::WAVES / 2; // uniform
+    const uint32_t tid = threadIdx.x % (32 * T::WAVES), piece = tid % LPR, sg = tid / LPR % 4, st = tid / LPR / 4;
+    u32x4 reg[8];
+    uint32_t pg[2]; // pages of the two blocks of 16 keys (loaded a tile ahead of the rows)
+    const uint8_t* vbase = (const uint8_t*)a.c.v;
+    const uint8_t* base = is_v ? vbase : (const uint8_t*)a.c.k;
+    // keys behind the range repeat its last one (masked below)
+    auto key_of = [&](uint32_t tile, uint32_t i) { return min(k_begin + BN * tile + 32 * st + (i / 4) * 16 + 4 * sg + i % 4, k_end - 1); };
+    auto pages = [&](uint32_t tile) {
+#pragma unroll
+        for (uint32_t b = 0; b < 2; b++) pg[b] = kv_page(a.c, u.seq, key_of(tile, 4 * b));
+    };
+    uint32_t bad_pages = 0; // of the tile in registers: bit b, this thread's block b has no page
+    auto fetch = [&](uint32_t tile) {
+        bad_pages = (pg[0] == KV_NO_PAGE ? 1u : 0u) | (pg[1] == KV_NO_PAGE ? 2u : 0u);
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i++) {
+            const uint32_t p = pg[i / 4] == KV_NO_PAGE ? 0u : pg[i / 4]; // without a page: page 0's row, masked
+            reg[i] = *(const u32x4*)(base + kv_row(a.c, p, kv, key_of(tile, i), DH) * T::ES + 16 * piece);
+        }
+    };
+    // whether every row of the block sees every key of a tile (pages aside)
+    auto tile_whole = [&](uint32_t tile) {
+        const uint32_t e = k_begin + BN * (tile + 1);
+        return e <= k_end && e <= u.pos + (TREE ? 0u : node0 + 1);
+    };
+    auto stage = [&](uint32_t tile, uint8_t* buf) {
+        uint8_t* s_k = buf;
+        uint8_t* s_v = buf + T::NH * T::KB;
+        float* s_e = (float*)(buf + T::NH * (T::KB + T::VB));
+        uint32_t* s_flag = (uint32_t*)(buf + T::NH * (T::KB + T::VB) + T::EXP);
+        const uint32_t kr = 32 * st + 4 * sg; // the row of key i is kr + 16 (i / 4) + i % 4
+        float sc[8];                          // what the rows are multiplied by (fp32)
+        uint32_t odd = 0; // bit i: value row i of this thread's eight holds something that is not finite (taken out here, added later)
+        if constexpr (F32) {
+            uint32_t mx[8], top[2];
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++)
+                mx[i] = max(max(reg[i][0] & 0x7FFFFFFFu, reg[i][1] & 0x7FFFFFFFu), max(reg[i][2] & 0x7FFFFFFFu, reg[i][3] & 0x7FFFFFFFu));
+            rows_max<LPR>(mx, top);
+            if (is_v && __builtin_amdgcn_ballot_w64(max(top[0], top[1]) >= 0x7F800000u)) { // rare: uniform
+#pragma unroll
+                for (uint32_t i = 0; i < 8; i++) {
+                    mx[i] = 0;
+                    bool bad = false;
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; j++) {
+                        const uint32_t x = reg[i][j];
+                        const bool nf = (x & 0x7F800000u) == 0x7F800000u;
+                        bad = bad || nf;
+                        reg[i][j] = nf ? 0u : x;
+                        mx[i] = max(mx[i], nf ? 0u : x & 0x7FFFFFFFu);
+                    }
+                    const uint64_t who = __builtin_amdgcn_ballot_w64(bad) >> (lane - piece % 64);
+                    odd |= ((LPR == 64 ? who : who & ((1ull << (LPR % 64)) - 1)) ? 1u : 0u) << i;
+                }
+                rows_max<LPR>(mx, top);
+            }
+            float sc2[2];
+#pragma unroll
+            for (uint32_t k = 0; k < 2; k++) {
+                const int e = max(top_exponent(u2f(top[k])), is_v ? TL_VMIN : -126);
+                sc2[k] = pow2i(-e);
+                if (piece < 4) { // row 4 k + piece of the eight
+                    float* at = s_e + kr + 16 * k + piece;
+                    if (is_v) {
+                        at[BN] = (float)e;
+                        at[2 * BN] = sc2[k];
+                    } else at[0] = pow2i(e);
+                }
+            }
+            quad_spread(sc2, sc);
+        } else if (is_v && (!tile_whole(tile) || __builtin_amdgcn_ballot_w64(bad_pages != 0))) { // uniform
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) {
+                bool bad = false;
+#pragma unroll
+                for (uint32_t j = 0; j < 4; j++) {
+                    const uint32_t x = reg[i][j];
+                    const bool b0 = (x & 0x7C00u) == 0x7C00u, b1 = (x & 0x7C000000u) == 0x7C000000u;
+                    bad = bad || b0 || b1;
+                    reg[i][j] = (b0 ? 0u : x & 0xFFFFu) | (b1 ? 0u : x & 0xFFFF0000u);
+                }
+                const uint64_t who = __builtin_amdgcn_ballot_w64(bad) >> (lane - piece);
+                odd |= ((who & ((1ull << LPR) - 1)) ? 1u : 0u) << i;
+            }
+        }
+        if (is_v) {
+            uint8_t* at = s_v + piece * T::VP + 64 * st + 16 * sg;
+#pragma unroll
+            for (uint32_t e = 0; e < E; e++, at += LPR * T::VP) {
+                if constexpr (F32) {
+                    float y[8];
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; i++) y[i] = u2f(reg[i][e]) * sc[i];
+                    const Half2 sp = split2(y);
+                    *(lds_u32x4*)at = __builtin_bit_cast(u32x4, sp.hi);
+                    *(lds_u32x4*)(at + T::VB) = __builtin_bit_cast(u32x4, sp.lo);
+                } else {
+                    u32x4 w;
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; i++) // half e of keys 2 i, 2 i + 1
+                        w[i] = __builtin_amdgcn_perm(reg[2 * i + 1][e / 2], reg[2 * i][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
+                    *(lds_u32x4*)at = w;
+                }
+            }
+            if (piece == 0) s_flag[sg * NB + st] = odd | bad_pages << 8;
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) {
+                uint8_t* at = s_k + (kr + 16 * (i / 4) + i % 4) * T::KP + (F32 ? 8 : 16) * piece;
+                if constexpr (F32) {
+                    float y[4];
+#pragma unroll
+                    for (uint32_t j = 0; j < 4; j++) y[j] = u2f(reg[i][j]) * sc[i];
+                    const uint32_t h0 = pack_half(y[0], y[1]), h1 = pack_half(y[2], y[3]);
+                    const half2v a0 = __builtin_bit_cast(half2v, h0), a1 = __builtin_bit_cast(half2v, h1);
+                    *(lds_u32x2*)at = u32x2{h0, h1};
+                    *(lds_u32x2*)(at + T::KB) = u32x2{pack_half(y[0] - (float)a0[0], y[1] - (float)a0[1]), pack_half(y[2] - (float)a1[0], y[3] - (float)a1[1])};
+                } else *(lds_u32x4*)at = reg[i];
+            }
+        }
+    };
+    // Scores, softmax and values of a tile's 32 keys from 32 sp for this wave.  whole: every row sees every key.  flagged: a page is
+    // missing or a value is not finite (never whole).
+    auto work = [&](uint32_t tile, const uint8_t* buf, bool whole, bool flagged, uint32_t sp) {
+        const uint8_t* s_k = buf;
+        const uint8_t* s_v = buf + T::NH * T::KB;
+        const float* s_e = (const float*)(buf + T::NH * (T::KB + T::VB));
+        const uint32_t* s_flag = (const uint32_t*)(buf + T::NH * (T::KB + T::VB) + T::EXP);
+        const uint32_t key0 = k_begin + BN * tile + 32 * sp;
+        float4v s[RT][2];
+#pragma unroll
+        for (uint32_t b = 0; b < 2; b++) {
+#pragma unroll
+            for (uint32_t rt = 0; rt < RT; rt++) s[rt][b] = float4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (uint32_t ks = 0; ks < KS; ks++) {
+                const uint8_t* at = s_k + (32 * sp + 16 * b + m) * T::KP + 64 * ks + 16 * g;
+                const half8 kh = __builtin_bit_cast(half8, u32x4(*(const lds_u32x4*)at));
+                if constexpr (F32) {
+                    const half8 kl = __builtin_bit_cast(half8, u32x4(*(const lds_u32x4*)(at + T::KB)));
+#pragma unroll
+                    for (uint32_t rt = 0; rt < RT; rt++) s[rt][b] = mfma16x32(kl, qh[rt][ks], s[rt][b]);
+                }
+#pragma unroll
+                for (uint32_t rt = 0; rt < RT; rt++) s[rt][b] = mfma16x32(kh, ql[rt][ks], s[rt][b]);
+#pragma unroll
+                for (uint32_t rt = 0; rt < RT; rt++) s[rt][b] = mfma16x32(kh, qh[rt][ks], s[rt][b]);
+            }
+        }
+        // scores in the log2 domain: this lane's row wr + 16 rt + m, keys 16 b + 4 g + r
+#pragma unroll
+        for (uint32_t b = 0; b < 2; b++) {
+            f32x4 kf, ve;
+            if constexpr (F32) {
+                const uint32_t j = 32 * sp + 16 * b + 4 * g;
+                kf = *(const lds_f32x4*)(s_e + j);
+                ve = *(const lds_f32x4*)(s_e + BN + j);
+            }
+#pragma unroll
+            for (uint32_t r = 0; r < 4; r++) {
+#pragma unroll
+                for (uint32_t rt = 0; rt < RT; rt++) {
+                    if constexpr (F32) s[rt][b][r] = s[rt][b][r] * (kf[r] * q_fac[rt]) + ve[r];
+                    else s[rt][b][r] *= q_fac[rt];
+                }
+            }
+        }
+        uint32_t seen = 0xFFFFu; // bit 8 rt + 4 b + r: the row sees that key
+        if (!whole) { // uniform
+            seen = 0;
+#pragma unroll
+            for (uint32_t rt = 0; rt < RT; rt++) {
+#pragma unroll
+                for (uint32_t b = 0; b < 2; b++) { // four neighbouring keys at a time
+                    const uint32_t key = key0 + 16 * b + 4 * g;
+                    const uint32_t bad = s_flag[sp] >> (8 + b) & 1u; // the first lane group's word of this step: its blocks without a page
+                    const uint32_t node = nodes >> (8 * rt) & 0xFFu;
+                    const uint32_t stop = bad || node == 0xFFu ? 0u : TREE ? k_end : min(k_end, u.pos + node0 + node + 1);
+                    uint32_t four = (1u << (stop > key ? min(stop - key, 4u) : 0u)) - 1u;
+                    if (TREE) four &= tree_four(s_kin[min(node, TL_M - 1)], (int32_t)(key - u.pos));
+                    seen |= four << (8 * rt + 4 * b);
+#pragma unroll
+                    for (uint32_t r = 0; r < 4; r++) s[rt][b][r] = (four >> r) & 1u ? s[rt][b][r] : -INFINITY;
+                }
+            }
+        }
+        float mx[RT];
+        bool over = false;
+#pragma unroll
+        for (uint32_t rt = 0; rt < RT; rt++) {
+            mx[rt] = AR_FLOOR;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; i++) mx[rt] = fmaxf(mx[rt], s[rt][i / 4][i % 4]);
+            over = over || mx[rt] > m_run[rt] + TL_SLACK;
+        }
+        if (__builtin_amdgcn_ballot_w64(over)) { // uniform: now and then
+#pragma unroll
+            for (uint32_t rt = 0; rt < RT; rt++) {
+                const float top = xor_lanes_max(mx[rt]), m_new = top > m_run[rt] + TL_SLACK ? top : m_run[rt];
+                const float corr = __builtin_amdgcn_exp2f(m_run[rt] - m_new);
+                m_run[rt] = m_new;
+                l_run[rt] *= corr;
+#pragma unroll
+                for (uint32_t n = 0; n < NT; n++) o[rt][n] *= corr;
+            }
+        }
+        half8 ph[RT], pl[RT];
+#pragma unroll
+        for (uint32_t rt = 0; rt < RT; rt++) {
+            const float top = m_run[rt] - TL_UP;
+            float sum = 0.f, p[8];
+#pragma unroll
+            for (uint32_t b = 0; b < 2; b++) {
+                f32x4 vi;
+                if constexpr (F32) vi = *(const lds_f32x4*)(s_e + 2 * BN + 32 * sp + 16 * b + 4 * g);
+#pragma unroll
+                for (uint32_t r = 0; r < 4; r++) {
+                    p[4 * b + r] = __builtin_amdgcn_exp2f(s[rt][b][r] - top);
+                    if constexpr (F32) sum += p[4 * b + r] * vi[r];
+                    else sum += p[4 * b + r];
+                }
+            }
+            l_run[rt] += sum; // of this lane's keys; the lane groups are added at the end
+            const Half2 p2 = split2(p);
+            ph[rt] = p2.hi;
+            pl[rt] = p2.lo;
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < NT; n++) {
+            const uint8_t* at = s_v + (16 * n + m) * T::VP + 64 * sp + 16 * g;
+            const half8 vh = __builtin_bit_cast(half8, u32x4(*(const lds_u32x4*)at));
+            if constexpr (F32) {
+                const half8 vl = __builtin_bit_cast(half8, u32x4(*(const lds_u32x4*)(at + T::VB)));
+#pragma unroll
+                for (uint32_t rt = 0; rt < RT; rt++) o[rt][n] = mfma16x32(vl, ph[rt], o[rt][n]);
+            }
+#pragma unroll
+            for (uint32_t rt = 0; rt < RT; rt++) o[rt][n] = mfma16x32(vh, pl[rt], o[rt][n]);
+#pragma unroll
+            for (uint32_t rt = 0; rt < RT; rt++) o[rt][n] = mfma16x32(vh, ph[rt], o[rt][n]);
+        }
+        if (flagged) { // rare: values that are not finite reach the rows that see them
+            for (uint32_t kk = 0; kk < 32; kk++) {
+                const uint32_t w = kk % 16 / 4, i = kk / 16 * 4 + kk % 4, key = key0 + kk; // the lane group that holds key kk, its place there
+                if (!((s_flag[w * NB + sp] >> i) & 1u) || key >= k_end) continue; // uniform
+                const uint32_t page = kv_page(a.c, u.seq, key);
+                if (page == KV_NO_PAGE) continue; // uniform
+                const uint8_t* row = vbase + kv_row(a.c, page, kv, key, DH) * T::ES;
+                for (uint32_t rt = 0; rt < RT; rt++) {
+                    const bool sees = ((uint32_t)__shfl((int)seen, (int)(16 * w + m)) >> (8 * rt + i)) & 1u;
+#pragma unroll
+                    for (uint32_t n = 0; n < NT; n++) {
+                        __builtin_amdgcn_sched_barrier(0); // registers: not all loads at once
+#pragma unroll
+                        for (uint32_t r = 0; r < 4; r++) {
+                            const uint32_t d = E * (16 * (n % NC) + 4 * g + r) + n / NC;
+                            const float v = F32 ? ((const float*)row)[d] : (float)((const _Float16*)row)[d];
+                            const float add = sees && !(fabsf(v) < INFINITY) ? v : 0.f;
+                            if (rt == 0) o[0][n][r] += add;
+                            else o[RT - 1][n][r] += add;
+                        }
+                    }
+                }
+            }
+        }
+    };
+
+    pages(0);
+    fetch(0);
+    if (n_tile > 1) pages(1);
+    stage(0, s_dyn);
+    if (n_tile > 1) fetch(1);
+    if (n_tile > 2) pages(2);
+    __syncthreads();
+    for (uint32_t tile = 0; tile < n_tile; tile++) {
+        const uint8_t* buf = s_dyn + (tile & 1u) * T::BUF;
+        const uint32_t* s_flag = (const uint32_t*)(buf + T::NH * (T::KB + T::VB) + T::EXP);
+        const uint32_t key0 = k_begin + BN * tile;
+        // the wave's rows see a prefix up to pos + node: nothing of this tile, all of it, or part
+        const bool flagged = __builtin_amdgcn_ballot_w64(lane < 4 * NB && s_flag[min(lane, 4 * NB - 1)] != 0) != 0;
+        const bool whole = !flagged && key0 + BN <= k_end && key0 + BN <= u.pos + (TREE ? 0u : first_node + 1); // uniform
+        if (has && key0 <= u.pos + last_node) { // uniform
+#pragma unroll
+            for (uint32_t sp = 0; sp < NB; sp++) work(tile, buf, whole, flagged, sp);
+        }
+        if (tile + 1 < n_tile) {
+            stage(tile + 1, s_dyn + ((tile + 1) & 1u) * T::BUF);
+            if (tile + 2 < n_tile) fetch(tile + 2);
+            if (tile + 3 < n_tile) pages(tile + 3);
+        }
+        __syncthreads();
+    }
+    if (!has) return; // the whole wave; no barrier below
+#pragma unroll
+    for (uint32_t rt = 0; rt < RT; rt++) {
+        const float l = xor_lanes_sum(l_run[rt]);
+        const uint32_t f = wr + 16 * rt + m;
+        if (f >= nr) continue;
+        const size_t rh = (size_t)(u.r0 + (f0 + f) / a.G) * a.hQ + kv * a.G + (f0 + f) % a.G;
+        const float inv = a.n_split > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        float* out = a.n_split > 1 ? a.acc + (rh * a.n_split + split) * DH : a.att + rh * DH;
+        if (a.n_split > 1 && g == 0) {
+            a.ml[2 * (rh * a.n_split + split)] = m_run[rt];
+            a.ml[2 * (rh * a.n_split + split) + 1] = l;
+        }
+#pragma unroll
+        for (uint32_t c = 0; c < NC; c++)
+#pragma unroll
+            for (uint32_t r = 0; r < 4; r++)
+#pragma unroll
+                for (uint32_t e = 0; e < E; e += 4) {
+                    const uint32_t d = E * (16 * c + 4 * g + r) + e;
+                    f32x4 x;
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; i++) x[i] = o[rt][(e + i) * NC + c][r] * inv;
+                    if (a.n_split == 1 && a.qfull) {
+                        const f32x4 gt = *(const f32x4*)(a.qfull + rh * 2 * DH + DH + d);
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; i++) x[i] *= 1.f / (1.f + expf(-gt[i]));
+                    }
+                    *(f32x4*)(out + d) = x;
+                }
+    }
+}
+
+template <int DH, bool F32, bool TREE>
+static void launch_tile(const RunsCall& a, hipStream_t st)
+{
+    constexpr uint32_t lds = 2 * TileGeom<DH, F32>::BUF;
+    static_assert(lds <= 160 * 1024, "LDS");
+    static bool once = ((void)hipFuncSetAttribute((const void*)attn_tile_kernel<DH, F32, TREE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), true);
+    (void)once;
+    hipLaunchKernelGGL((attn_tile_kernel<DH, F32, TREE>), dim3(tile_blocks(a.R.n_rows, a.R.n_run, a.G) * a.c.n_kv * a.n_split), dim3(64 * TileGeom<DH, F32>::WAVES), lds, st, a);
+}
+
+void launch_attn_tile(const RunsCall& a, int type, uint32_t dh, bool tree, hipStream_t st)
+{
+    if (dh == 256) {
+        if (type == QKK_F32) tree ? launch_tile<256, true, true>(a, st) : launch_tile<256, true, false>(a, st);
+        else tree ? launch_tile<256, false, true>(a, st) : launch_tile<256, false, false>(a, st);
+    } else {
+        if (type == QKK_F32) tree ? launch_tile<128, true, true>(a, st) : launch_tile<128, true, false>(a, st);
+        else tree ? launch_tile<128, false, true>(a, st) : launch_tile<128, false, false>(a, st);
+    }
+}
+
+} // namespace qk
