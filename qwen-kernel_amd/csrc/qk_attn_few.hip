@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256, (DH == 128 && RT == 1 ? 2 : 1)) void attn_few_
     __shared__ float s_m[2][RT * 16], s_l[2][RT * 16];
     __shared__ int32_t s_up[TREE ? QKK_TREE_MAX : 1];
     __shared__ uint32_t s_kin[TREE ? RT * 16 : 1][QKK_TREE_MAX / 32];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, m = lane & 15u, g = lane >> 4;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15u, g = lane >> 4;
     // Workgroups go to the eight dies in turn, so the KV head and the run vary fastest: every die gets the same share of the first
     // ranges, which every run has, and of the last ones, which few have (with the range varying fastest one die had all the first).
     const uint32_t kv = blockIdx.x % a.c.n_kv, run = blockIdx.x / a.c.n_kv % a.R.n_run, split = blockIdx.x / a.c.n_kv / a.R.n_run;
@@ -70,18 +70,17 @@ __global__ __launch_bounds__(256, (DH == 128 && RT == 1 ? 2 : 1)) void attn_few_
     const uint8_t* kbase = (const uint8_t*)a.c.k;
     const uint8_t* vbase = (const uint8_t*)a.c.v;
     constexpr uint32_t ES = F32 ? 4 : 2;
-    // the pages of a step's blocks of 16 keys (a page holds a multiple of 16 rows; a slot cache is one page)
+    // the page ids of a step's blocks of 16 keys (a page holds a multiple of 16 rows; a slot cache is one page), requested a step ahead of
+    // the rows and not looked at before; behind the last step the last block's again
     auto pages = [&](uint32_t step, uint32_t* pg) {
 #pragma unroll
-        for (uint32_t b = 0; b < 2 * SUB; b++) {
-            const uint32_t key = k_begin + SK * step + 16 * b;
-            pg[b] = key < k_end ? kv_page(a.c, u.seq, key) : KV_NO_PAGE;
-        }
+        for (uint32_t b = 0; b < 2 * SUB; b++) pg[b] = (uint32_t)*kv_page_at(a.c, a.R.seq + run, u.seq, min(k_begin + SK * step + 16 * b, k_end - 1));
     };
+    auto valid = [&](uint32_t step, uint32_t b, const uint32_t* pg) { return pg[b] < a.c.n_page && k_begin + SK * step + 16 * b < k_end; };
     // block b of K.  Rows behind the range repeat its last one (masked below); without a page, and behind the last step: zeros, no load
     auto fetch_k = [&](uint32_t step, uint32_t b, const uint32_t* pg) {
         const uint32_t key = min(k_begin + SK * step + 16 * b + m, k_end - 1);
-        if (pg[b] != KV_NO_PAGE) { // uniform
+        if (valid(step, b, pg)) { // uniform
             const uint8_t* row = kbase + kv_row(a.c, pg[b], kv, key, DH) * ES;
 #pragma unroll
             for (uint32_t ks = 0; ks < KS; ks++)
@@ -99,7 +98,7 @@ __global__ __launch_bounds__(256, (DH == 128 && RT == 1 ? 2 : 1)) void attn_few_
 #pragma unroll
         for (uint32_t i = 0; i < 8; i++) {
             const uint32_t b = 2 * sb + i / 4, key = min(k_begin + SK * step + 16 * b + 4 * g + i % 4, k_end - 1);
-            if (pg[b] != KV_NO_PAGE) { // uniform
+            if (valid(step, b, pg)) { // uniform
                 const uint8_t* row = vbase + kv_row(a.c, pg[b], kv, key, DH) * ES;
 #pragma unroll
                 for (uint32_t c = c0; c < c1; c++) vreg[sb][c][i] = *(const u32x4*)(row + (c * 16 + m) * 16);
@@ -228,7 +227,7 @@ __global__ __launch_bounds__(256, (DH == 128 && RT == 1 ? 2 : 1)) void attn_few_
         // softmax: this lane's row 16 rt + m, keys 16 b + 4 g + r
         bool whole = key0 + SK <= k_end && key0 + SK <= u.pos + (TREE ? 0u : 1u); // uniform
 #pragma unroll
-        for (uint32_t b = 0; b < 2 * SUB; b++) whole = whole && pg[b] != KV_NO_PAGE;
+        for (uint32_t b = 0; b < 2 * SUB; b++) whole = whole && pg[b] < a.c.n_page;
         uint32_t seen[RT]; // bit 4 b + r: the row sees that key
         Bf3 p3[RT][SUB];
         Half2 p2[RT][SUB];
@@ -244,7 +243,7 @@ __global__ __launch_bounds__(256, (DH == 128 && RT == 1 ? 2 : 1)) void attn_few_
 #pragma unroll
                 for (uint32_t b = 0; b < 2 * SUB; b++) { // four neighbouring keys at a time
                     const uint32_t key = key0 + 16 * b + 4 * g;
-                    const uint32_t stop = pg[b] == KV_NO_PAGE || f >= nr ? 0u : TREE ? k_end : min(k_end, u.pos + node + 1);
+                    const uint32_t stop = pg[b] >= a.c.n_page || f >= nr ? 0u : TREE ? k_end : min(k_end, u.pos + node + 1);
                     uint32_t four = (1u << (stop > key ? min(stop - key, 4u) : 0u)) - 1u;
                     if (drafts) four &= tree_four(s_kin[node], (int32_t)(key - u.pos));
                     seen[rt] |= four << (4 * b);

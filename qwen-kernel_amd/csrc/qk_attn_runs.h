@@ -85,20 +85,38 @@ __device__ __forceinline__ Bf3 split3(const float* x)
     return r;
 }
 
-// Eight floats as hi + lo halves, both rounded to nearest: exact to 2^-22 of x while x is inside a half's normal range.
+// Eight floats as hi + lo halves, both rounded to nearest: exact to 2^-22 of x while x is inside a half's normal range.  Two values
+// take three instructions: one packs both hi halves, and the rest x * s - hi is formed and rounded by one mixed-precision
+// multiply-add each.  The pinned register keeps the compiler from converting every value a second time on its own, the pinned
+// factor 1 from turning the multiply-add into a subtraction of converted values.
 struct Half2 {
     half8 hi, lo;
 };
 __device__ __forceinline__ uint32_t pack_half(float a, float b) { return __builtin_bit_cast(uint32_t, half2v{(_Float16)a, (_Float16)b}); }
+__device__ __forceinline__ float pinned_one()
+{
+    float one = 1.f;
+    asm("" : QK_REG(one));
+    return one;
+}
+__device__ __forceinline__ void split_pair(float a, float b, float s, bool scaled, uint32_t& hi, uint32_t& lo)
+{
+    uint32_t top = scaled ? pack_half(a * s, b * s) : pack_half(a, b);
+    asm("" : QK_REG(top));
+    const half2v h = __builtin_bit_cast(half2v, top);
+    hi = top;
+    lo = __builtin_bit_cast(uint32_t, half2v{(_Float16)__builtin_fmaf(a, s, -(float)h[0]), (_Float16)__builtin_fmaf(b, s, -(float)h[1])});
+}
 __device__ __forceinline__ Half2 split2(const float* x)
 {
     u32x4 h, l;
+    const float one = pinned_one();
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const uint32_t top = pack_half(x[2 * i], x[2 * i + 1]);
-        const half2v hv = __builtin_bit_cast(half2v, top);
-        h[i] = top;
-        l[i] = pack_half(x[2 * i] - (float)hv[0], x[2 * i + 1] - (float)hv[1]);
+        uint32_t hi, lo;
+        split_pair(x[2 * i], x[2 * i + 1], one, false, hi, lo);
+        h[i] = hi;
+        l[i] = lo;
     }
     return Half2{__builtin_bit_cast(half8, h), __builtin_bit_cast(half8, l)};
 }

@@ -5,9 +5,11 @@
 // Q operand and its accumulators in registers: two waves per SIMD, so one's softmax runs beside another's products.  A
 // tile of 32 (fp32) or 64 (half) keys goes from the cache to registers while the tile before it is worked on -- half of the waves
 // load K, the others V -- and from there to the other one of two LDS buffers:
-//   K    as it lies, [key][dim] halves (row pitch + 16 bytes: 16 lanes fall on 16 different bank groups);
-//   V^T  [dim][key]: a thread holds 8 keys x 4 (fp32) or 8 (half) dims, in the order of keys that the weights P have in the
-//        registers of the first product, and writes 16 bytes per dim.
+// Both operands lie in LDS in the order in which the matrix instruction's lanes read them, 64 x 16 bytes per fragment, so reads are
+// linear and free of bank conflicts (rows with 16 bytes of padding lost a fifth of the time to them):
+//   K    fragments [block of 16 keys][step of 32 dims]; a thread stages pieces of one or two rows;
+//   V^T  fragments [block of 16 dims][step of 32 keys]; a thread stages 8 keys x 4 (fp32) or 8 (half) dims, in the order of keys
+//        that the weights P have in the registers of the first product, 16 bytes per dim.
 // One barrier per tile.  Matrix work per key and row: 4 dh operations times the products of split operands.
 //   F16 cache   K and V are operands as they are, Q and P are hi + lo halves: two products.
 //   F32 cache   every row of K and V is divided by the power of two that brings its largest value into [1, 2) and split
@@ -37,12 +39,17 @@ struct TileGeom {
     static constexpr uint32_t RT = TL_M / WAVES / 16;              // blocks of 16 rows per wave
     static constexpr uint32_t LPR = DH * ES / 16;                  // 16-byte pieces of a row = lanes that load one
     static constexpr uint32_t NB = F32 ? 1 : 2, BN = 32 * NB;      // steps of 32 keys per tile
-    static constexpr uint32_t KP = DH * 2 + 16, VP = NB * 64 + 16; // row pitches, bytes
-    static constexpr uint32_t KB = BN * KP, VB = DH * VP;          // one copy of K, of V^T
+    static constexpr uint32_t KB = BN * DH * 2, VB = KB;           // bytes of one copy of K, of V^T
+    static constexpr uint32_t RL = F32 ? 8 : 16, QL = 64 / RL;     // staging K: rows, and pieces of each, per wave and load
+    static constexpr uint32_t PI = LPR / QL, KR = 8 / PI;          // loads per row, rows per thread
     static constexpr uint32_t EXP = F32 ? 3 * BN * 4 : 0;          // per key: factor of the score, exponent and factor of the value row
     static constexpr uint32_t BUF = NH * (KB + VB) + EXP + 64;     // + flags [4 NB]
+    // Operand fragments read ahead of the products, and whether that order is pinned: left to itself the scheduler keeps two in flight,
+    // which costs dh 256 4 % and suits halves with dh 128; fp32 with dh 128 has registers for one only.
+    static constexpr uint32_t AHEAD = DH == 256 ? 3 : 1;
+    static constexpr bool PIN = DH == 256 || F32;
     // half of the waves stage K, the others V: eight pieces per thread
-    static_assert(NB * LPR * 4 == WAVES * 32, "staging");
+    static_assert(NB * LPR * 4 == WAVES * 32 && WAVES / 2 * RL * KR == BN, "staging");
 };
 
 // Maxima of eight rows' magnitudes (as integers, so NaN counts as the largest) over the LPR lanes that hold a row: after the
@@ -94,7 +101,7 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
     QK_DYN_LDS(uint8_t, s_dyn);
     __shared__ int32_t s_up[TREE ? QKK_TREE_MAX : 1];
     __shared__ uint32_t s_kin[TREE ? TL_M : 1][QKK_TREE_MAX / 32];
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, m = lane & 15u, g = lane >> 4;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15u, g = lane >> 4;
 
     // workgroup -> KV head, block of rows (the last, longest ones first), range of keys.  Workgroups go to the eight dies in turn: with
     // the range varying slowest every die gets its share of the first ranges, which every block has.  A run's blocks begin at its
@@ -164,27 +171,51 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
     for (uint32_t rt = 0; rt < RT; rt++) nodes |= (wr + 16 * rt + m < nr ? (f0 + wr + 16 * rt + m) / a.G - node0 : 0xFFu) << (8 * rt);
     const uint32_t first_node = (f0 + min(wr, nr - 1)) / a.G, last_node = (f0 + min(wr + WR, nr) - 1) / a.G;
 
-    // Staging: the first half of the waves takes V, the second K.  A thread: (piece of a row, lane group sg of the second
-    // product, step of 32 keys st), its eight keys of that step 4 sg + i and 16 + 4 sg + i.
+    // Which of the four keys from `key` on this lane's row of block rt sees, pages aside.
+    auto sees = [&](uint32_t rt, uint32_t key) {
+        const uint32_t node = nodes >> (8 * rt) & 0xFFu;
+        const uint32_t stop = node == 0xFFu ? 0u : TREE ? k_end : min(k_end, u.pos + node0 + node + 1);
+        uint32_t four = (1u << (stop > key ? min(stop - key, 4u) : 0u)) - 1u;
+        if (TREE) four &= k_end > u.pos ? tree_four(s_kin[min(node, TL_M - 1)], (int32_t)(key - u.pos)) : 15u;
+        return four;
+    };
+    bool odd_values = false; // uniform: some value of this range is not finite
+
+    // Staging: the first half of the waves takes V, the second K, eight 16-byte pieces per thread.
+    //   V  (piece, lane group sg of the second product, step st of 32 keys): keys 4 sg + i and 16 + 4 sg + i of the step, i < 4
+    //   K  rows RL (KR kw + j) + kr of the tile, j < KR, pieces kq + QL i, i < PI (kw: the wave among those that stage K)
     const bool is_v = wave < T::WAVES / 2; // uniform
     const uint32_t tid = threadIdx.x % (32 * T::WAVES), piece = tid % LPR, sg = tid / LPR % 4, st = tid / LPR / 4;
+    const uint32_t kr = lane % T::RL, kq = lane / T::RL, k_row0 = (wave % (T::WAVES / 2)) * T::RL * T::KR + kr;
+    // A thread's pieces lie in two groups of four, each at one distance from the next -- V rows 4 sg .. 4 sg + 3 of a block of 16 keys, which
+    // are neighbours in their page, or four pieces of one K row -- so a tile takes two full addresses (64-bit products are
+    // slow), not eight.  Keys behind the range repeat its last one (masked below).
     u32x4 reg[8];
-    uint32_t pg[2]; // pages of the two blocks of 16 keys (loaded a tile ahead of the rows)
     const uint8_t* vbase = (const uint8_t*)a.c.v;
-    const uint8_t* base = is_v ? vbase : (const uint8_t*)a.c.k;
-    // keys behind the range repeat its last one (masked below)
-    auto key_of = [&](uint32_t tile, uint32_t i) { return min(k_begin + BN * tile + 32 * st + (i / 4) * 16 + 4 * sg + i % 4, k_end - 1); };
+    const uint8_t* kbase = (const uint8_t*)a.c.k;
+    const uint32_t stride = is_v ? DH * T::ES : 16 * T::QL; // uniform
+    auto first_key = [&](uint32_t tile, uint32_t b) {
+        uint32_t key = 32 * st + 16 * b + 4 * sg;
+        if (!is_v) key = k_row0 + (T::KR == 1 ? 0 : T::RL * b);
+        return min(k_begin + BN * tile + key, k_end - 1);
+    };
+    uint32_t pg[2]; // the groups' page ids, requested a tile ahead of the rows and not looked at before
     auto pages = [&](uint32_t tile) {
 #pragma unroll
-        for (uint32_t b = 0; b < 2; b++) pg[b] = kv_page(a.c, u.seq, key_of(tile, 4 * b));
+        for (uint32_t b = 0; b < 2; b++) pg[b] = (uint32_t)*kv_page_at(a.c, a.R.seq + run, u.seq, first_key(tile, b));
     };
-    uint32_t bad_pages = 0; // of the tile in registers: bit b, this thread's block b has no page
+    const float one = pinned_one();
+    uint32_t bad_pages = 0; // of the tile in registers: bit b, this thread's group b has no page
     auto fetch = [&](uint32_t tile) {
-        bad_pages = (pg[0] == KV_NO_PAGE ? 1u : 0u) | (pg[1] == KV_NO_PAGE ? 2u : 0u);
+        bad_pages = (pg[0] >= a.c.n_page ? 1u : 0u) | (pg[1] >= a.c.n_page ? 2u : 0u);
 #pragma unroll
-        for (uint32_t i = 0; i < 8; i++) {
-            const uint32_t p = pg[i / 4] == KV_NO_PAGE ? 0u : pg[i / 4]; // without a page: page 0's row, masked
-            reg[i] = *(const u32x4*)(base + kv_row(a.c, p, kv, key_of(tile, i), DH) * T::ES + 16 * piece);
+        for (uint32_t b = 0; b < 2; b++) {
+            const uint32_t key = first_key(tile, b), p = pg[b] >= a.c.n_page ? 0u : pg[b]; // without a page: page 0's row, masked
+            const size_t at = kv_row(a.c, p, kv, key, DH) * T::ES + 16 * (is_v ? piece : kq + (T::KR == 1 ? 4 * T::QL * b : 0));
+            const uint8_t* row = (is_v ? vbase : kbase) + at;
+            const uint32_t lim = is_v ? k_end - 1 - key : 3u; // V: rows behind the first that are inside the range
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) reg[4 * b + i] = *(const u32x4*)(row + min(i, lim) * stride);
         }
     };
     // whether every row of the block sees every key of a tile (pages aside)
@@ -197,8 +228,40 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
         uint8_t* s_v = buf + T::NH * T::KB;
         float* s_e = (float*)(buf + T::NH * (T::KB + T::VB));
         uint32_t* s_flag = (uint32_t*)(buf + T::NH * (T::KB + T::VB) + T::EXP);
-        const uint32_t kr = 32 * st + 4 * sg; // the row of key i is kr + 16 (i / 4) + i % 4
-        float sc[8];                          // what the rows are multiplied by (fp32)
+        if (!is_v) {
+#pragma unroll
+            for (uint32_t j = 0; j < T::KR; j++) {
+                const uint32_t row = k_row0 + T::RL * j;
+                uint8_t* at = s_k + (row / 16 * KS * 64 + row % 16) * 16;
+                if constexpr (F32) {
+                    float mx = 0.f; // NaN is passed over here and stays one in its key's scores
+#pragma unroll
+                    for (uint32_t i = 0; i < T::PI; i++)
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(u2f(reg[T::PI * j + i][e])));
+                    mx = fmaxf(mx, dpp_f<0x128>(mx)); // the row's eight lanes: lane % 8 is the row (row_ror 8)
+                    mx = xor_lanes_max(mx);
+                    const int ex = top_exponent(mx);
+                    const float scale = pow2i(-ex);
+                    if (kq == 0) s_e[row] = pow2i(ex);
+                    at += kq / 2 * 256 + kq % 2 * 8;
+#pragma unroll
+                    for (uint32_t i = 0; i < T::PI; i++) { // pieces kq + 8 i: step i of 32 dims
+                        const u32x4 x = reg[T::PI * j + i];
+                        uint32_t h0, h1, l0, l1;
+                        split_pair(u2f(x[0]), u2f(x[1]), scale, true, h0, l0);
+                        split_pair(u2f(x[2]), u2f(x[3]), scale, true, h1, l1);
+                        *(lds_u32x2*)(at + 1024 * i) = u32x2{h0, h1};
+                        *(lds_u32x2*)(at + 1024 * i + T::KB) = u32x2{l0, l1};
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t i = 0; i < T::PI; i++) *(lds_u32x4*)(at + kq * 256 + 1024 * i) = reg[T::PI * j + i];
+                }
+            }
+            return;
+        }
+        float sc[8];      // what the value rows are multiplied by (fp32)
         uint32_t odd = 0; // bit i: value row i of this thread's eight holds something that is not finite (taken out here, added later)
         if constexpr (F32) {
             uint32_t mx[8], top[2];
@@ -206,7 +269,7 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
             for (uint32_t i = 0; i < 8; i++)
                 mx[i] = max(max(reg[i][0] & 0x7FFFFFFFu, reg[i][1] & 0x7FFFFFFFu), max(reg[i][2] & 0x7FFFFFFFu, reg[i][3] & 0x7FFFFFFFu));
             rows_max<LPR>(mx, top);
-            if (is_v && __builtin_amdgcn_ballot_w64(max(top[0], top[1]) >= 0x7F800000u)) { // rare: uniform
+            if (__builtin_amdgcn_ballot_w64(max(top[0], top[1]) >= 0x7F800000u)) { // rare: uniform
 #pragma unroll
                 for (uint32_t i = 0; i < 8; i++) {
                     mx[i] = 0;
@@ -227,18 +290,16 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
             float sc2[2];
 #pragma unroll
             for (uint32_t k = 0; k < 2; k++) {
-                const int e = max(top_exponent(u2f(top[k])), is_v ? TL_VMIN : -126);
+                const int e = max(top_exponent(u2f(top[k])), TL_VMIN);
                 sc2[k] = pow2i(-e);
                 if (piece < 4) { // row 4 k + piece of the eight
-                    float* at = s_e + kr + 16 * k + piece;
-                    if (is_v) {
-                        at[BN] = (float)e;
-                        at[2 * BN] = sc2[k];
-                    } else at[0] = pow2i(e);
+                    float* at = s_e + 32 * st + 4 * sg + 16 * k + piece;
+                    at[BN] = (float)e;
+                    at[2 * BN] = sc2[k];
                 }
             }
             quad_spread(sc2, sc);
-        } else if (is_v && (!tile_whole(tile) || __builtin_amdgcn_ballot_w64(bad_pages != 0))) { // uniform
+        } else if (!tile_whole(tile) || __builtin_amdgcn_ballot_w64(bad_pages != 0)) { // uniform
 #pragma unroll
             for (uint32_t i = 0; i < 8; i++) {
                 bool bad = false;
@@ -253,45 +314,33 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
                 odd |= ((who & ((1ull << LPR) - 1)) ? 1u : 0u) << i;
             }
         }
-        if (is_v) {
-            uint8_t* at = s_v + piece * T::VP + 64 * st + 16 * sg;
+        // dim E piece + e is row piece % 16 of block NC e + piece / 16
+        uint8_t* at = s_v + (((piece / 16) * NB + st) * 64 + 16 * sg + piece % 16) * 16;
 #pragma unroll
-            for (uint32_t e = 0; e < E; e++, at += LPR * T::VP) {
-                if constexpr (F32) {
-                    float y[8];
+        for (uint32_t e = 0; e < E; e++, at += NC * NB * 1024) {
+            u32x4 w;
+            if constexpr (F32) {
+                u32x4 lo;
 #pragma unroll
-                    for (uint32_t i = 0; i < 8; i++) y[i] = u2f(reg[i][e]) * sc[i];
-                    const Half2 sp = split2(y);
-                    *(lds_u32x4*)at = __builtin_bit_cast(u32x4, sp.hi);
-                    *(lds_u32x4*)(at + T::VB) = __builtin_bit_cast(u32x4, sp.lo);
-                } else {
-                    u32x4 w;
-#pragma unroll
-                    for (uint32_t i = 0; i < 4; i++) // half e of keys 2 i, 2 i + 1
-                        w[i] = __builtin_amdgcn_perm(reg[2 * i + 1][e / 2], reg[2 * i][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
-                    *(lds_u32x4*)at = w;
+                for (uint32_t i = 0; i < 4; i++) {
+                    // two keys, each with its own factor: scaled first
+                    uint32_t h, l;
+                    split_pair(u2f(reg[2 * i][e]) * sc[2 * i], u2f(reg[2 * i + 1][e]) * sc[2 * i + 1], one, false, h, l);
+                    w[i] = h;
+                    lo[i] = l;
                 }
-            }
-            if (piece == 0) s_flag[sg * NB + st] = odd | bad_pages << 8;
-        } else {
+                *(lds_u32x4*)(at + T::VB) = lo;
+            } else {
 #pragma unroll
-            for (uint32_t i = 0; i < 8; i++) {
-                uint8_t* at = s_k + (kr + 16 * (i / 4) + i % 4) * T::KP + (F32 ? 8 : 16) * piece;
-                if constexpr (F32) {
-                    float y[4];
-#pragma unroll
-                    for (uint32_t j = 0; j < 4; j++) y[j] = u2f(reg[i][j]) * sc[i];
-                    const uint32_t h0 = pack_half(y[0], y[1]), h1 = pack_half(y[2], y[3]);
-                    const half2v a0 = __builtin_bit_cast(half2v, h0), a1 = __builtin_bit_cast(half2v, h1);
-                    *(lds_u32x2*)at = u32x2{h0, h1};
-                    *(lds_u32x2*)(at + T::KB) = u32x2{pack_half(y[0] - (float)a0[0], y[1] - (float)a0[1]), pack_half(y[2] - (float)a1[0], y[3] - (float)a1[1])};
-                } else *(lds_u32x4*)at = reg[i];
+                for (uint32_t i = 0; i < 4; i++) // half e of keys 2 i, 2 i + 1
+                    w[i] = __builtin_amdgcn_perm(reg[2 * i + 1][e / 2], reg[2 * i][e / 2], e % 2 ? 0x07060302u : 0x05040100u);
             }
+            *(lds_u32x4*)at = w;
         }
+        if (piece == 0) s_flag[sg * NB + st] = odd | bad_pages << 8;
     };
-    // Scores, softmax and values of a tile's 32 keys from 32 sp for this wave.  whole: every row sees every key.  flagged: a page is
-    // missing or a value is not finite (never whole).
-    auto work = [&](uint32_t tile, const uint8_t* buf, bool whole, bool flagged, uint32_t sp) {
+    // Scores, softmax and values of a tile's 32 keys from 32 sp for this wave.  whole: every row sees every key.
+    auto work = [&](uint32_t tile, const uint8_t* buf, bool whole, uint32_t sp) {
         const uint8_t* s_k = buf;
         const uint8_t* s_v = buf + T::NH * T::KB;
         const float* s_e = (const float*)(buf + T::NH * (T::KB + T::VB));
@@ -299,24 +348,36 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
         const uint32_t key0 = k_begin + BN * tile + 32 * sp;
         float4v s[RT][2];
 #pragma unroll
-        for (uint32_t b = 0; b < 2; b++) {
+        for (uint32_t b = 0; b < 2; b++)
 #pragma unroll
             for (uint32_t rt = 0; rt < RT; rt++) s[rt][b] = float4v{0.f, 0.f, 0.f, 0.f};
+        half8 fh[T::AHEAD], fl[T::AHEAD];
+        auto read = [&](const uint8_t* at, uint32_t copy, uint32_t slot) {
+            fh[slot] = __builtin_bit_cast(half8, u32x4(*(const lds_u32x4*)at));
+            if constexpr (F32) fl[slot] = __builtin_bit_cast(half8, u32x4(*(const lds_u32x4*)(at + copy)));
+        };
+        const uint8_t* kf_at = s_k + (2 * sp * KS * 64 + lane) * 16;
 #pragma unroll
-            for (uint32_t ks = 0; ks < KS; ks++) {
-                const uint8_t* at = s_k + (32 * sp + 16 * b + m) * T::KP + 64 * ks + 16 * g;
-                const half8 kh = __builtin_bit_cast(half8, u32x4(*(const lds_u32x4*)at));
-                if constexpr (F32) {
-                    const half8 kl = __builtin_bit_cast(half8, u32x4(*(const lds_u32x4*)(at + T::KB)));
+        for (uint32_t i = 0; i < T::AHEAD; i++) read(kf_at + 1024 * i, T::KB, i);
+        if (T::PIN) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (uint32_t rt = 0; rt < RT; rt++) s[rt][b] = mfma16x32(kl, qh[rt][ks], s[rt][b]);
-                }
+        for (uint32_t i = 0; i < 2 * KS; i++) {
+            const uint32_t b = i / KS, ks = i % KS, slot = i % T::AHEAD;
+            if constexpr (F32) {
 #pragma unroll
-                for (uint32_t rt = 0; rt < RT; rt++) s[rt][b] = mfma16x32(kh, ql[rt][ks], s[rt][b]);
-#pragma unroll
-                for (uint32_t rt = 0; rt < RT; rt++) s[rt][b] = mfma16x32(kh, qh[rt][ks], s[rt][b]);
+                for (uint32_t rt = 0; rt < RT; rt++) s[rt][b] = mfma16x32(fl[slot], qh[rt][ks], s[rt][b]);
             }
+#pragma unroll
+            for (uint32_t rt = 0; rt < RT; rt++) s[rt][b] = mfma16x32(fh[slot], ql[rt][ks], s[rt][b]);
+#pragma unroll
+            for (uint32_t rt = 0; rt < RT; rt++) s[rt][b] = mfma16x32(fh[slot], qh[rt][ks], s[rt][b]);
+            if (i + T::AHEAD < 2 * KS) read(kf_at + 1024 * (i + T::AHEAD), T::KB, slot);
+            if (T::PIN) __builtin_amdgcn_sched_barrier(0);
         }
+        const uint8_t* vf_at = s_v + (sp * 64 + lane) * 16;
+#pragma unroll
+        for (uint32_t i = 0; i < T::AHEAD; i++) read(vf_at + 1024 * NB * i, T::VB, i); // the first values arrive during the softmax
+        if (T::PIN) __builtin_amdgcn_sched_barrier(0);
         // scores in the log2 domain: this lane's row wr + 16 rt + m, keys 16 b + 4 g + r
 #pragma unroll
         for (uint32_t b = 0; b < 2; b++) {
@@ -335,20 +396,14 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
                 }
             }
         }
-        uint32_t seen = 0xFFFFu; // bit 8 rt + 4 b + r: the row sees that key
         if (!whole) { // uniform
-            seen = 0;
 #pragma unroll
             for (uint32_t rt = 0; rt < RT; rt++) {
 #pragma unroll
                 for (uint32_t b = 0; b < 2; b++) { // four neighbouring keys at a time
                     const uint32_t key = key0 + 16 * b + 4 * g;
                     const uint32_t bad = s_flag[sp] >> (8 + b) & 1u; // the first lane group's word of this step: its blocks without a page
-                    const uint32_t node = nodes >> (8 * rt) & 0xFFu;
-                    const uint32_t stop = bad || node == 0xFFu ? 0u : TREE ? k_end : min(k_end, u.pos + node0 + node + 1);
-                    uint32_t four = (1u << (stop > key ? min(stop - key, 4u) : 0u)) - 1u;
-                    if (TREE) four &= tree_four(s_kin[min(node, TL_M - 1)], (int32_t)(key - u.pos));
-                    seen |= four << (8 * rt + 4 * b);
+                    const uint32_t four = bad ? 0u : sees(rt, key);
 #pragma unroll
                     for (uint32_t r = 0; r < 4; r++) s[rt][b][r] = (four >> r) & 1u ? s[rt][b][r] : -INFINITY;
                 }
@@ -395,43 +450,20 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
             ph[rt] = p2.hi;
             pl[rt] = p2.lo;
         }
+        if (T::PIN) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (uint32_t n = 0; n < NT; n++) {
-            const uint8_t* at = s_v + (16 * n + m) * T::VP + 64 * sp + 16 * g;
-            const half8 vh = __builtin_bit_cast(half8, u32x4(*(const lds_u32x4*)at));
+            const uint32_t slot = n % T::AHEAD;
             if constexpr (F32) {
-                const half8 vl = __builtin_bit_cast(half8, u32x4(*(const lds_u32x4*)(at + T::VB)));
 #pragma unroll
-                for (uint32_t rt = 0; rt < RT; rt++) o[rt][n] = mfma16x32(vl, ph[rt], o[rt][n]);
+                for (uint32_t rt = 0; rt < RT; rt++) o[rt][n] = mfma16x32(fl[slot], ph[rt], o[rt][n]);
             }
 #pragma unroll
-            for (uint32_t rt = 0; rt < RT; rt++) o[rt][n] = mfma16x32(vh, pl[rt], o[rt][n]);
+            for (uint32_t rt = 0; rt < RT; rt++) o[rt][n] = mfma16x32(fh[slot], pl[rt], o[rt][n]);
 #pragma unroll
-            for (uint32_t rt = 0; rt < RT; rt++) o[rt][n] = mfma16x32(vh, ph[rt], o[rt][n]);
-        }
-        if (flagged) { // rare: values that are not finite reach the rows that see them
-            for (uint32_t kk = 0; kk < 32; kk++) {
-                const uint32_t w = kk % 16 / 4, i = kk / 16 * 4 + kk % 4, key = key0 + kk; // the lane group that holds key kk, its place there
-                if (!((s_flag[w * NB + sp] >> i) & 1u) || key >= k_end) continue; // uniform
-                const uint32_t page = kv_page(a.c, u.seq, key);
-                if (page == KV_NO_PAGE) continue; // uniform
-                const uint8_t* row = vbase + kv_row(a.c, page, kv, key, DH) * T::ES;
-                for (uint32_t rt = 0; rt < RT; rt++) {
-                    const bool sees = ((uint32_t)__shfl((int)seen, (int)(16 * w + m)) >> (8 * rt + i)) & 1u;
-#pragma unroll
-                    for (uint32_t n = 0; n < NT; n++) {
-                        __builtin_amdgcn_sched_barrier(0); // registers: not all loads at once
-#pragma unroll
-                        for (uint32_t r = 0; r < 4; r++) {
-                            const uint32_t d = E * (16 * (n % NC) + 4 * g + r) + n / NC;
-                            const float v = F32 ? ((const float*)row)[d] : (float)((const _Float16*)row)[d];
-                            const float add = sees && !(fabsf(v) < INFINITY) ? v : 0.f;
-                            if (rt == 0) o[0][n][r] += add;
-                            else o[RT - 1][n][r] += add;
-                        }
-                    }
-                }
-            }
+            for (uint32_t rt = 0; rt < RT; rt++) o[rt][n] = mfma16x32(fh[slot], ph[rt], o[rt][n]);
+            if (n + T::AHEAD < NT) read(vf_at + 1024 * NB * (n + T::AHEAD), T::VB, slot);
+            if (T::PIN) __builtin_amdgcn_sched_barrier(0);
         }
     };
 
@@ -447,11 +479,13 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
         const uint32_t* s_flag = (const uint32_t*)(buf + T::NH * (T::KB + T::VB) + T::EXP);
         const uint32_t key0 = k_begin + BN * tile;
         // the wave's rows see a prefix up to pos + node: nothing of this tile, all of it, or part
-        const bool flagged = __builtin_amdgcn_ballot_w64(lane < 4 * NB && s_flag[min(lane, 4 * NB - 1)] != 0) != 0;
+        const uint32_t flag = lane < 4 * NB ? s_flag[min(lane, 4 * NB - 1)] : 0u;
+        const bool flagged = __builtin_amdgcn_ballot_w64(flag != 0) != 0;
+        if (flagged) odd_values = odd_values || __builtin_amdgcn_ballot_w64((flag & 0xFFu) != 0) != 0;
         const bool whole = !flagged && key0 + BN <= k_end && key0 + BN <= u.pos + (TREE ? 0u : first_node + 1); // uniform
         if (has && key0 <= u.pos + last_node) { // uniform
 #pragma unroll
-            for (uint32_t sp = 0; sp < NB; sp++) work(tile, buf, whole, flagged, sp);
+            for (uint32_t sp = 0; sp < NB; sp++) work(tile, buf, whole, sp);
         }
         if (tile + 1 < n_tile) {
             stage(tile + 1, s_dyn + ((tile + 1) & 1u) * T::BUF);
@@ -461,6 +495,27 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
         __syncthreads();
     }
     if (!has) return; // the whole wave; no barrier below
+    if (odd_values) { // rare: values that are not finite were taken out of the products; they reach the rows that see them here
+        for (uint32_t key0 = k_begin; key0 < k_end; key0 += 4) { // from a multiple of four: one page
+            const uint32_t page = kv_page(a.c, u.seq, key0);
+            if (page == KV_NO_PAGE) continue; // uniform
+            for (uint32_t k = 0; k < 4 && key0 + k < k_end; k++) {
+                const uint8_t* row = vbase + kv_row(a.c, page, kv, key0 + k, DH) * T::ES;
+#pragma unroll
+                for (uint32_t n = 0; n < NT; n++) {
+                    __builtin_amdgcn_sched_barrier(0); // registers: not all loads at once
+#pragma unroll
+                    for (uint32_t r = 0; r < 4; r++) {
+                        const uint32_t d = E * (16 * (n % NC) + 4 * g + r) + n / NC;
+                        const float v = F32 ? ((const float*)row)[d] : (float)((const _Float16*)row)[d];
+#pragma unroll
+                        for (uint32_t rt = 0; rt < RT; rt++)
+                            if (!(fabsf(v) < INFINITY) && ((sees(rt, key0) >> k) & 1u)) o[rt][n][r] += v;
+                    }
+                }
+            }
+        }
+    }
 #pragma unroll
     for (uint32_t rt = 0; rt < RT; rt++) {
         const float l = xor_lanes_sum(l_run[rt]);

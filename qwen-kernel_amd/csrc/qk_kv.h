@@ -26,6 +26,13 @@ __device__ __forceinline__ uint32_t kv_page(const KvView& c, uint32_t seq, uint3
     const uint32_t p = c.table ? (uint32_t)c.table[(size_t)seq * c.seq_pages + (r >> c.shift)] : seq;
     return p < c.n_page ? p : KV_NO_PAGE;
 }
+// Where the page id of row r is to be read, for loops that request ids ahead of their use: to be compared with n_page THEN, since a
+// comparison here would wait for the load, and with it for every load in front of it.  seq_at holds the sequence's own id,
+// which is the page of a slot cache.
+__device__ __forceinline__ const int32_t* kv_page_at(const KvView& c, const int32_t* seq_at, uint32_t seq, uint32_t r)
+{
+    return c.table ? c.table + ((size_t)seq * c.seq_pages + (r >> c.shift)) : seq_at;
+}
 // Element offset of a row of KV head h in k or v (64 bits: a long cache passes 2^32 elements).
 __device__ __forceinline__ size_t kv_row(const KvView& c, uint32_t page, uint32_t h, uint32_t r, uint32_t dh)
 {

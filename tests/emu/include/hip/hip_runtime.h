@@ -297,6 +297,7 @@ emu_float4 emu_mfma_16x16x32_bf16(emu_bf16x8 a, emu_bf16x8 b, emu_float4 c);
 
 #define __builtin_amdgcn_update_dpp emu_update_dpp
 #define __builtin_amdgcn_readlane emu_readlane
+#define __builtin_amdgcn_readfirstlane(x) (x) // used on values that are the same in every lane
 #define __builtin_amdgcn_ds_bpermute emu_bpermute
 #define __builtin_amdgcn_ballot_w64 emu_ballot
 #define __builtin_amdgcn_fdot2 emu_fdot2
