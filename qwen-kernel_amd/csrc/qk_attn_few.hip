@@ -37,13 +37,14 @@ __global__ __launch_bounds__(256, (DH == 128 && RT == 1 ? 2 : 1)) void attn_few_
     __shared__ int32_t s_up[TREE ? QKK_TREE_MAX : 1];
     __shared__ uint32_t s_kin[TREE ? RT * 16 : 1][QKK_TREE_MAX / 32];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15u, g = lane >> 4;
-    // Workgroups go to the eight dies in turn, so the KV head and the run vary fastest: every die gets the same share of the first
-    // ranges, which every run has, and of the last ones, which few have (with the range varying fastest one die had all the first).
-    const uint32_t kv = blockIdx.x % a.c.n_kv, run = blockIdx.x / a.c.n_kv % a.R.n_run, split = blockIdx.x / a.c.n_kv / a.R.n_run;
-    const Run u = run_at(a.c, a.R, run);
-    const uint32_t nr = u.n * a.G, end = min(u.pos + u.n, a.c.cap), k_begin = split * a.chunk;
-    if (!u.ok || nr == 0 || k_begin >= end) return; // the whole workgroup
-    const uint32_t k_end = min(end, k_begin + a.chunk);
+    const uint32_t kv = blockIdx.x % a.c.n_kv;
+    const Item it = item_of(a, blockIdx.x / a.c.n_kv, RT * 16);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.n_split > 1) *a.chunk_used = it.chunk;
+    if (!it.ok) return; // the whole workgroup
+    const Run u = it.u;
+    const uint32_t run = it.run, split = it.split;
+    const uint32_t nr = u.n * a.G, end = min(u.pos + u.n, a.c.cap), k_begin = split * it.chunk;
+    const uint32_t k_end = min(end, k_begin + it.chunk);
     const bool drafts = TREE && k_end > u.pos; // uniform: this range holds rows of the tree itself
     int32_t up_of = -1;
     if (drafts) up_of = tree_parent(a.parent, u);
@@ -477,7 +478,7 @@ static void launch_few(const RunsCall& a, bool tree, hipStream_t st)
 {
     constexpr uint32_t q_bytes = (F32 ? 3 : 2) * RT * (DH / 32) * 1024, o_bytes = 2 * RT * 16 * (DH + 4) * 4;
     constexpr uint32_t lds = q_bytes > o_bytes ? q_bytes : o_bytes;
-    const dim3 grid(a.R.n_run * a.c.n_kv * a.n_split), block(256);
+    const dim3 grid(items_of(a.R.n_run, a.slots, a.n_split) * a.c.n_kv), block(256);
     if (tree) {
         static bool once = ((void)hipFuncSetAttribute((const void*)attn_few_kernel<DH, F32, RT, true>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), true);
         (void)once;

@@ -25,16 +25,80 @@ namespace qk {
 constexpr float AR_FLOOR = -3.0e38f;
 constexpr float AR_LOG2E = 1.44269504088896341f;
 
-// One call.  Keys are cut into ranges of `chunk` rows (a multiple of 128), n_split of them cover the cache; with n_split 1 the
-// kernels write att, else each range's (maximum, sum, weighted sum) go to the workspace and attn_join_kernel folds them.
+// One call.  With n_split 1 a workgroup takes all keys of its rows and writes att.  Else the keys are cut into ranges, each range's
+// (maximum, sum, weighted sum) go to the workspace and attn_join_kernel folds them.  How long a range is, is decided on the
+// device from the lengths (item_of), not below `chunk` (a multiple of 128), of which n_split cover the cache.
 struct RunsCall {
     KvView c;
     RunsView R;
     const int32_t* parent;
     const float *q, *qfull;
     float *att, *acc, *ml; // acc [row][head][n_split][dh], ml [row][head][n_split][2] (log2 domain)
-    uint32_t hQ, G, n_split, chunk;
+    uint32_t* chunk_used;  // one word of the workspace
+    uint32_t hQ, G, n_split, chunk, slots; // slots: items per KV head that fill the device
 };
+
+// The piece of work with number `item` of its KV head: a run, a block of its rows, a range of keys.
+struct Item {
+    Run u;
+    uint32_t run, block, split, chunk;
+    bool ok;
+};
+// Sequences of a batch differ in length by orders of magnitude, and the lengths live on the device.  Every wave looks all of them
+// over (64 runs per round trip), takes the range that cuts the whole of them -- blocks of `rows` rows times keys -- into as
+// many items as there are places on the device, and finds its own item by a prefix sum; items without work come last and end
+// at once.  (With ranges fixed by the host three of four workgroups of sixteen ragged sequences had no work, and those that had
+// some waited behind them: 37 us.)  Every workgroup comes to the same range; the join finds it in the workspace.
+__device__ __forceinline__ Item item_of(const RunsCall& a, uint32_t item, uint32_t rows)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    auto look = [&](uint32_t i, uint32_t& nb, uint32_t& end) {
+        nb = end = 0;
+        if (i >= a.R.n_run) return;
+        const Run u = run_at(a.c, a.R, i);
+        if (!u.ok || !u.n) return;
+        nb = (u.n * a.G + rows - 1) / rows;
+        end = min(u.pos + u.n, a.c.cap);
+    };
+    uint32_t nb0, end0, blocks = 0; // the first 64 runs stay in registers
+    uint64_t work = 0;              // in pieces of 64 keys
+    look(lane, nb0, end0);
+    for (uint32_t i = lane; i < a.R.n_run; i += 64) {
+        uint32_t nb = nb0, end = end0;
+        if (i != lane) look(i, nb, end);
+        blocks += nb;
+        work += (uint64_t)nb * ((end + 63) / 64);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        blocks += __shfl_xor(blocks, d);
+        work += __shfl_xor(work, d);
+    }
+    const uint64_t places = a.slots > 2 * blocks ? a.slots - blocks : max(blocks, 1u);
+    const uint64_t want = ((work + places - 1) / places * 64 + 127) / 128 * 128;
+    Item it;
+    it.chunk = __builtin_amdgcn_readfirstlane((uint32_t)min(max(want, (uint64_t)a.chunk), (uint64_t)1 << 30));
+    it.ok = false;
+    uint32_t before = 0;
+    for (uint32_t i0 = 0; i0 < a.R.n_run; i0 += 64) {
+        uint32_t nb = nb0, end = end0;
+        if (i0) look(i0 + lane, nb, end);
+        const uint32_t mine = nb * ((end + it.chunk - 1) / it.chunk), incl = before + wave_incl_scan_u32(mine);
+        const uint64_t past = __builtin_amdgcn_ballot_w64(incl > item);
+        if (past) {
+            const uint32_t at = (uint32_t)__builtin_ctzll(past);
+            const uint32_t first = (uint32_t)__shfl((int)(incl - mine), (int)at), splits = (uint32_t)__shfl((int)((end + it.chunk - 1) / it.chunk), (int)at);
+            it.run = __builtin_amdgcn_readfirstlane(i0 + at);
+            it.block = __builtin_amdgcn_readfirstlane((item - first) / splits);
+            it.split = __builtin_amdgcn_readfirstlane((item - first) % splits);
+            it.u = run_at(a.c, a.R, it.run);
+            it.ok = true;
+            return it;
+        }
+        before = (uint32_t)__shfl((int)incl, 63);
+    }
+    return it;
+}
 
 __device__ __forceinline__ float xor_lanes_max(float v) // over the four lane groups: lanes with the same lane % 16
 {
@@ -176,6 +240,14 @@ __device__ __forceinline__ uint32_t tree_four(const uint32_t* kin, int32_t rel)
 // at its own first row, so every run may have one that is not full
 constexpr uint32_t AR_TILE_ROWS = 128;
 inline uint32_t tile_blocks(uint32_t n_rows, uint32_t n_run, uint32_t G) { return (uint32_t)((uint64_t)n_rows * G / AR_TILE_ROWS) + n_run; }
+
+// Items of one KV head that a launch has to have room for, `blocks` the blocks of rows at most (item_of makes no more than `slots` of
+// them, or two per block): one per block where the keys are not cut.
+inline uint32_t items_of(uint32_t blocks, uint32_t slots, uint32_t n_split)
+{
+    const uint64_t all = (uint64_t)blocks * n_split, made = slots > 2 * blocks ? slots : 2ull * blocks;
+    return (uint32_t)(n_split == 1 ? blocks : all < made ? all : made);
+}
 
 void launch_attn_few(const RunsCall& call, int type, uint32_t dh, bool tree, hipStream_t st);
 void launch_attn_tile(const RunsCall& call, int type, uint32_t dh, bool tree, hipStream_t st);

@@ -22,7 +22,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(RunsCall a)
     if (ri >= a.R.n_run) return;
     const Run u = run_at(a.c, a.R, ri);
     if (!u.ok || row - u.r0 >= u.n) return;
-    const uint32_t n = (min(u.pos + (row - u.r0) + 1, a.c.cap) + a.chunk - 1) / a.chunk;
+    const uint32_t chunk = *a.chunk_used, n = (min(u.pos + (row - u.r0) + 1, a.c.cap) + chunk - 1) / chunk;
     const size_t rh = (size_t)row * a.hQ + h, at = rh * a.n_split;
     float m = AR_FLOOR, l = 0.f;
     if (lane < n) {
@@ -58,10 +58,10 @@ __global__ __launch_bounds__(256) void attn_join_kernel(RunsCall a)
 }
 
 // How a call is cut, from what the host knows (never from the lengths, which live on the device, so that a captured launch
-// follows them): which kernel, and the ranges of keys that run in parallel.
+// follows them): which kernel, and how short the ranges of keys that run in parallel may get.  The workspace is sized by it.
 struct Plan {
     bool few;
-    uint32_t n_split, chunk;
+    uint32_t n_split, chunk, slots;
 };
 static Plan plan_of(const qkk_kv_cache* C, const qkk_kv_runs* R, uint32_t hQ)
 {
@@ -69,19 +69,18 @@ static Plan plan_of(const qkk_kv_cache* C, const qkk_kv_runs* R, uint32_t hQ)
     const uint64_t cap = (uint64_t)C->seq_pages * C->page_rows;
     Plan p;
     p.few = (uint64_t)max_run * G <= few_rows(C->dh);
+    // places on the device: two workgroups per CU (256) where registers and LDS allow two
+    const bool two = C->dh == 128 && (!p.few || (uint64_t)max_run * G <= 16);
+    p.slots = std::max(1u, (two ? 512u : 256u) / C->n_kv);
+    uint64_t ranges = 64; // at most: the join's lanes
     if (!p.few) {
-        // one range where the blocks of rows fill the chip (one workgroup per CU), else about two workgroups per CU
+        // one range where the blocks of rows fill the chip, else no more than two per place: the partial results are memory, too
         const uint64_t groups = std::max<uint64_t>(((uint64_t)R->n_rows * G + AR_TILE_ROWS - 1) / AR_TILE_ROWS, R->n_run) * C->n_kv;
-        const uint64_t ranges = groups >= 256 ? 1 : std::min<uint64_t>(64, (512 + groups - 1) / groups);
-        p.chunk = (uint32_t)std::max<uint64_t>(128, ((cap + ranges - 1) / ranges + 127) / 128 * 128);
-        p.n_split = (uint32_t)((cap + p.chunk - 1) / p.chunk);
-        return p;
+        ranges = groups >= 256 ? 1 : std::min<uint64_t>(64, (1024 + groups - 1) / groups);
     }
-    // ranges of one step per wave (128 keys, 256 for halves with dh 128) while about two thousand workgroups cover the whole cache
-    // with them, longer ones beyond; at most 64 (the join's lanes)
-    const uint64_t units = (uint64_t)R->n_run * C->n_kv, step = C->type == QKK_F16 && C->dh == 128 ? 256 : 128;
-    const uint64_t want = std::max((cap * units + 2047) / 2048, (cap + 63) / 64);
-    p.chunk = (uint32_t)std::max<uint64_t>(step, (want + step - 1) / step * step);
+    // a range is at least one step per wave (128 keys; 256 for few rows on halves with dh 128)
+    const uint64_t step = p.few && C->type == QKK_F16 && C->dh == 128 ? 256 : 128;
+    p.chunk = (uint32_t)std::max<uint64_t>(step, ((cap + ranges - 1) / ranges + step - 1) / step * step);
     p.n_split = (uint32_t)((cap + p.chunk - 1) / p.chunk);
     return p;
 }
@@ -104,7 +103,7 @@ static int attn_runs(const char* who, const qkk_kv_cache* C, uint32_t layer, con
     if (int rc = require_device()) return rc;
     if (!runs.n_rows || !runs.n_run) return QKK_OK;
     const Plan plan = plan_of(C, R, hQ);
-    if ((uint64_t)(tile_blocks(runs.n_rows, runs.n_run, hQ / c.n_kv)) * c.n_kv * plan.n_split > (1u << 30) || (uint64_t)runs.n_rows * hQ > (1u << 30))
+    if (2 * (uint64_t)(tile_blocks(runs.n_rows, runs.n_run, hQ / c.n_kv)) * c.n_kv > (1u << 30) || (uint64_t)runs.n_rows * hQ > (1u << 30))
         return fail(QKK_ESHAPE, "%s: rows x heads or runs x heads too large", who);
     {
         RunsCall a;
@@ -120,6 +119,8 @@ static int attn_runs(const char* who, const qkk_kv_cache* C, uint32_t layer, con
         a.G = hQ / c.n_kv;
         a.n_split = plan.n_split;
         a.chunk = plan.chunk;
+        a.slots = plan.slots;
+        a.chunk_used = (uint32_t*)(a.ml + 2 * (size_t)runs.n_rows * hQ * plan.n_split);
         if (plan.few) launch_attn_few(a, C->type, C->dh, tree, as_stream(stream));
         else launch_attn_tile(a, C->type, C->dh, tree, as_stream(stream));
         if (plan.n_split > 1) {

@@ -103,23 +103,37 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
     __shared__ uint32_t s_kin[TREE ? TL_M : 1][QKK_TREE_MAX / 32];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15u, g = lane >> 4;
 
-    // workgroup -> KV head, block of rows (the last, longest ones first), range of keys.  Workgroups go to the eight dies in turn: with
-    // the range varying slowest every die gets its share of the first ranges, which every block has.  A run's blocks begin at its
-    // own first row; run i's first block has the number floor(start G / 128) + i, which leaves every run room for its
-    // last, part-filled one.
-    const uint32_t n_blocks = gridDim.x / a.c.n_kv / a.n_split;
-    const uint32_t kv = blockIdx.x % a.c.n_kv, blk = n_blocks - 1 - blockIdx.x / a.c.n_kv % n_blocks, split = blockIdx.x / a.c.n_kv / n_blocks;
-    auto first_of = [&](uint32_t i) { return (int64_t)((uint64_t)max(a.R.start[i], 0) * a.G / TL_M) + i; };
-    const uint32_t run = wave_last_le(a.R.n_run, blk, first_of);
-    if (run >= a.R.n_run) return; // the whole workgroup
-    const Run u = run_at(a.c, a.R, run);
-    const uint32_t f0 = (blk - (uint32_t)first_of(run)) * TL_M, rows_all = u.n * a.G;
+    // workgroup -> KV head (neighbours differ in it: they run on different dies, which then keep one head's cache in their L2), run,
+    // block of rows, range of keys
+    const uint32_t kv = blockIdx.x % a.c.n_kv;
+    uint32_t run, f0, split = 0, chunk = a.c.cap;
+    Run u;
+    if (a.n_split == 1) {
+        // the last (longest) blocks first.  A run's blocks begin at its own first row; run i's first block has the number
+        // floor(start G / 128) + i, which leaves every run room for its last, part-filled one.
+        const uint32_t blk = gridDim.x / a.c.n_kv - 1 - blockIdx.x / a.c.n_kv;
+        auto first_of = [&](uint32_t i) { return (int64_t)((uint64_t)max(a.R.start[i], 0) * a.G / TL_M) + i; };
+        run = wave_last_le(a.R.n_run, blk, first_of);
+        if (run >= a.R.n_run) return; // the whole workgroup
+        u = run_at(a.c, a.R, run);
+        f0 = (blk - (uint32_t)first_of(run)) * TL_M;
+    } else {
+        const Item it = item_of(a, blockIdx.x / a.c.n_kv, TL_M);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *a.chunk_used = it.chunk;
+        if (!it.ok) return; // the whole workgroup
+        u = it.u;
+        run = it.run;
+        f0 = it.block * TL_M;
+        split = it.split;
+        chunk = it.chunk;
+    }
+    const uint32_t rows_all = u.n * a.G;
     if (!u.ok || f0 >= rows_all) return; // the whole workgroup
     const uint32_t nr = min(TL_M, rows_all - f0);
     const uint32_t last = (f0 + nr - 1) / a.G; // the block's last position in the run
-    const uint32_t end = min(u.pos + last + 1, a.c.cap), k_begin = split * a.chunk;
+    const uint32_t end = min(u.pos + last + 1, a.c.cap), k_begin = split * chunk;
     if (k_begin >= end) return; // the whole workgroup
-    const uint32_t k_end = min(end, k_begin + a.chunk), n_tile = (k_end - k_begin + BN - 1) / BN;
+    const uint32_t k_end = min(end, k_begin + chunk), n_tile = (k_end - k_begin + BN - 1) / BN;
     const uint32_t node0 = f0 / a.G;
     if (TREE && k_end > u.pos) tree_bits(tree_parent(a.parent, u), node0, last - node0 + 1, s_up, s_kin);
 
@@ -204,7 +218,6 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
 #pragma unroll
         for (uint32_t b = 0; b < 2; b++) pg[b] = (uint32_t)*kv_page_at(a.c, a.R.seq + run, u.seq, first_key(tile, b));
     };
-    const float one = pinned_one();
     uint32_t bad_pages = 0; // of the tile in registers: bit b, this thread's group b has no page
     auto fetch = [&](uint32_t tile) {
         bad_pages = (pg[0] >= a.c.n_page ? 1u : 0u) | (pg[1] >= a.c.n_page ? 2u : 0u);
@@ -315,6 +328,7 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
             }
         }
         // dim E piece + e is row piece % 16 of block NC e + piece / 16
+        const float one = pinned_one();
         uint8_t* at = s_v + (((piece / 16) * NB + st) * 64 + 16 * sg + piece % 16) * 16;
 #pragma unroll
         for (uint32_t e = 0; e < E; e++, at += NC * NB * 1024) {
@@ -555,7 +569,7 @@ static void launch_tile(const RunsCall& a, hipStream_t st)
     static_assert(lds <= 160 * 1024, "LDS");
     static bool once = ((void)hipFuncSetAttribute((const void*)attn_tile_kernel<DH, F32, TREE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), true);
     (void)once;
-    hipLaunchKernelGGL((attn_tile_kernel<DH, F32, TREE>), dim3(tile_blocks(a.R.n_rows, a.R.n_run, a.G) * a.c.n_kv * a.n_split), dim3(64 * TileGeom<DH, F32>::WAVES), lds, st, a);
+    hipLaunchKernelGGL((attn_tile_kernel<DH, F32, TREE>), dim3(items_of(tile_blocks(a.R.n_rows, a.R.n_run, a.G), a.slots, a.n_split) * a.c.n_kv), dim3(64 * TileGeom<DH, F32>::WAVES), lds, st, a);
 }
 
 void launch_attn_tile(const RunsCall& a, int type, uint32_t dh, bool tree, hipStream_t st)
