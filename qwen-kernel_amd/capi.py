@@ -571,12 +571,11 @@ def _want(who, name, t, dtype, shape, dev):
 
 
 def _here(who, dev):
-    """The calls go to the current device's current stream: the cache has to be there.  Returns that stream."""
+    """The calls go to the current device's current stream: the cache has to be there."""
     if dev >= 0:
         import torch
         if dev != torch.cuda.current_device():
             raise ValueError(f"{who}: the cache is on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
-    return _stream()
 
 
 def _bytes(who, t, dev):
@@ -656,7 +655,7 @@ def attn_prep_axes(cache, layer, runs, q, kin, vin, q_norm_w, k_norm_w, rope, pa
     _, hQ, pitch = q.shape
     rope_rows, half, _ = rope.shape
     n_axis = axis_pos.shape[0]
-    stream = _here(who, dev)
+    _here(who, dev)
     _same_device(who, cache, runs)
     if qhat is None:
         qhat = q.new_empty((rows, hQ, dh))
@@ -666,7 +665,7 @@ def attn_prep_axes(cache, layer, runs, q, kin, vin, q_norm_w, k_norm_w, rope, pa
         _want(who, "vin", vin, f, kv, dev), _want(who, "q_norm_w", q_norm_w, f, w, dev), _want(who, "k_norm_w", k_norm_w, f, w, dev),
         _want(who, "rope", rope, f, None, dev), rope_rows, _want(who, "pair_axis", pair_axis, cache.u8, (half,), dev), n_axis,
         _want(who, "axis_pos", axis_pos, cache.i32, (n_axis, rows), dev), _want(who, "qhat", qhat, f, (rows, hQ, dh), dev), hQ, 2 * half,
-        int(pitch != dh), eps, stream))
+        int(pitch != dh), eps, _stream()))
     return qhat
 
 
@@ -679,7 +678,7 @@ def _attn_runs(who, cache, layer, runs, parent, qhat, workspace, qfull, att):
     if qhat.dim() != 3:
         raise ValueError(f"{who}: qhat must be [rows][hQ][dh]")
     hQ = qhat.shape[1]
-    stream = _here(who, dev)
+    _here(who, dev)
     _same_device(who, cache, runs)
     if att is None:
         att = qhat.new_empty((rows, hQ, dh))
@@ -688,10 +687,10 @@ def _attn_runs(who, cache, layer, runs, parent, qhat, workspace, qfull, att):
     gate = 0 if qfull is None else _want(who, "qfull", qfull, f, (rows, hQ, 2 * dh), dev)
     space, nbytes = _bytes(who, workspace, dev)
     if parent is None:
-        _check(lib().qkk_attn_packed(cache.ref_c, layer, runs.ref_c, q, gate, out, space, nbytes, hQ, stream))
+        _check(lib().qkk_attn_packed(cache.ref_c, layer, runs.ref_c, q, gate, out, space, nbytes, hQ, _stream()))
     else:
         up = _want(who, "parent", parent, cache.i32, (rows,), dev)
-        _check(lib().qkk_attn_tree(cache.ref_c, layer, runs.ref_c, up, q, gate, out, space, nbytes, hQ, stream))
+        _check(lib().qkk_attn_tree(cache.ref_c, layer, runs.ref_c, up, q, gate, out, space, nbytes, hQ, _stream()))
     return att
 
 
@@ -717,12 +716,12 @@ def kv_resize(cache, len_new, workspace, status=None):
     """Sets the rows each sequence holds (int32 [n_seq]; -1: as it is, 0: freed); pages are freed and taken, a shared part-filled page is
     copied before its sequence grows.  Returns the device status word: 0, the number of missing pages (nothing grew), or -1."""
     who, dev = "kv_resize", cache.dev
-    stream = _here(who, dev)
+    _here(who, dev)
     if status is None:
         status = len_new.new_empty((1,))
     space, nbytes = _bytes(who, workspace, dev)
     _check(lib().qkk_kv_resize(cache.ref_c, _want(who, "len_new", len_new, cache.i32, (cache.n_seq,), dev),
-                               _want(who, "status", status, cache.i32, (1,), dev), space, nbytes, stream))
+                               _want(who, "status", status, cache.i32, (1,), dev), space, nbytes, _stream()))
     return status
 
 
@@ -730,12 +729,12 @@ def kv_fork(cache, src, dst, workspace, status=None):
     """Sequences dst (empty) get the rows of src, sharing their pages (a slot cache: copies of the rows).  Returns the device status
     word: 0, or -1 where nothing was changed."""
     who, dev, n = "kv_fork", cache.dev, src.numel()
-    stream = _here(who, dev)
+    _here(who, dev)
     if status is None:
         status = src.new_empty((1,))
     space, nbytes = _bytes(who, workspace, dev)
     _check(lib().qkk_kv_fork(cache.ref_c, _want(who, "src", src, cache.i32, (n,), dev), _want(who, "dst", dst, cache.i32, (n,), dev), n,
-                             _want(who, "status", status, cache.i32, (1,), dev), space, nbytes, stream))
+                             _want(who, "status", status, cache.i32, (1,), dev), space, nbytes, _stream()))
     return status
 
 
@@ -745,7 +744,7 @@ def kv_compact(cache, seq, base, path, n_path):
     who, dev, i32, n = "kv_compact", cache.dev, cache.i32, seq.numel()
     if path.dim() != 2:
         raise ValueError("kv_compact: path must be [n][max_path]")
-    stream = _here(who, dev)
+    _here(who, dev)
     wide = path.shape[1]
     _check(lib().qkk_kv_compact(cache.ref_c, _want(who, "seq", seq, i32, (n,), dev), _want(who, "base", base, i32, (n,), dev),
-                                _want(who, "path", path, i32, (n, wide), dev), _want(who, "n_path", n_path, i32, (n,), dev), n, wide, stream))
+                                _want(who, "path", path, i32, (n, wide), dev), _want(who, "n_path", n_path, i32, (n,), dev), n, wide, _stream()))

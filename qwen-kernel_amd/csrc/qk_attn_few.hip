@@ -39,7 +39,6 @@ __global__ __launch_bounds__(256, (DH == 128 && RT == 1 ? 2 : 1)) void attn_few_
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15u, g = lane >> 4;
     const uint32_t kv = blockIdx.x % a.c.n_kv;
     const Item it = item_of(a, blockIdx.x / a.c.n_kv, RT * 16);
-    if (blockIdx.x == 0 && threadIdx.x == 0 && a.n_split > 1) *a.chunk_used = it.chunk;
     if (!it.ok) return; // the whole workgroup
     const Run u = it.u;
     const uint32_t run = it.run, split = it.split;

@@ -27,7 +27,7 @@ constexpr float AR_LOG2E = 1.44269504088896341f;
 
 // One call.  With n_split 1 a workgroup takes all keys of its rows and writes att.  Else the keys are cut into ranges, each range's
 // (maximum, sum, weighted sum) go to the workspace and attn_join_kernel folds them.  How long a range is, is decided on the
-// device from the lengths (item_of), not below `chunk` (a multiple of 128), of which n_split cover the cache.
+// device from the lengths (item_of), a multiple of `grain` and not below `chunk`, of which n_split cover the cache.
 struct RunsCall {
     KvView c;
     RunsView R;
@@ -35,7 +35,7 @@ struct RunsCall {
     const float *q, *qfull;
     float *att, *acc, *ml; // acc [row][head][n_split][dh], ml [row][head][n_split][2] (log2 domain)
     uint32_t* chunk_used;  // one word of the workspace
-    uint32_t hQ, G, n_split, chunk, slots; // slots: items per KV head that fill the device
+    uint32_t hQ, G, n_split, chunk, grain, slots; // slots: items per KV head that fill the device
 };
 
 // The piece of work with number `item` of its KV head: a run, a block of its rows, a range of keys.
@@ -47,8 +47,14 @@ struct Item {
 // Sequences of a batch differ in length by orders of magnitude, and the lengths live on the device.  Every wave looks all of them
 // over (64 runs per round trip), takes the range that cuts the whole of them -- blocks of `rows` rows times keys -- into as
 // many items as there are places on the device, and finds its own item by a prefix sum; items without work come last and end
-// at once.  (With ranges fixed by the host three of four workgroups of sixteen ragged sequences had no work, and those that had
-// some waited behind them: 37 us.)  Every workgroup comes to the same range; the join finds it in the workspace.
+// at once.  A run's own ranges are then made equal.  (With ranges fixed by the host three of four workgroups of sixteen ragged sequences had no work, and those that had
+// some waited behind them: 37 us.)  Every workgroup comes to the same result; the join finds the common range in the workspace.
+// The length of a run's ranges, all but the last: as many as `chunk` makes, of one length.
+__device__ __forceinline__ uint32_t run_chunk(uint32_t end, uint32_t chunk, uint32_t grain)
+{
+    const uint32_t splits = max((end + chunk - 1) / chunk, 1u), each = (end + splits - 1) / splits;
+    return max((each + grain - 1) / grain, 1u) * grain;
+}
 __device__ __forceinline__ Item item_of(const RunsCall& a, uint32_t item, uint32_t rows)
 {
     const uint32_t lane = threadIdx.x & 63u;
@@ -75,22 +81,25 @@ __device__ __forceinline__ Item item_of(const RunsCall& a, uint32_t item, uint32
         work += __shfl_xor(work, d);
     }
     const uint64_t places = a.slots > 2 * blocks ? a.slots - blocks : max(blocks, 1u);
-    const uint64_t want = ((work + places - 1) / places * 64 + 127) / 128 * 128;
+    const uint64_t want = ((work + places - 1) / places * 64 + a.grain - 1) / a.grain * a.grain;
     Item it;
-    it.chunk = __builtin_amdgcn_readfirstlane((uint32_t)min(max(want, (uint64_t)a.chunk), (uint64_t)1 << 30));
+    const uint32_t chunk = __builtin_amdgcn_readfirstlane((uint32_t)min(max(want, (uint64_t)a.chunk), (uint64_t)1 << 30));
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.n_split > 1) *a.chunk_used = chunk;
     it.ok = false;
     uint32_t before = 0;
     for (uint32_t i0 = 0; i0 < a.R.n_run; i0 += 64) {
         uint32_t nb = nb0, end = end0;
         if (i0) look(i0 + lane, nb, end);
-        const uint32_t mine = nb * ((end + it.chunk - 1) / it.chunk), incl = before + wave_incl_scan_u32(mine);
+        const uint32_t mine = nb * ((end + chunk - 1) / chunk), incl = before + wave_incl_scan_u32(mine);
         const uint64_t past = __builtin_amdgcn_ballot_w64(incl > item);
         if (past) {
             const uint32_t at = (uint32_t)__builtin_ctzll(past);
-            const uint32_t first = (uint32_t)__shfl((int)(incl - mine), (int)at), splits = (uint32_t)__shfl((int)((end + it.chunk - 1) / it.chunk), (int)at);
+            const uint32_t first = (uint32_t)__shfl((int)(incl - mine), (int)at), last = (uint32_t)__shfl((int)end, (int)at);
+            const uint32_t splits = (last + chunk - 1) / chunk;
             it.run = __builtin_amdgcn_readfirstlane(i0 + at);
             it.block = __builtin_amdgcn_readfirstlane((item - first) / splits);
             it.split = __builtin_amdgcn_readfirstlane((item - first) % splits);
+            it.chunk = __builtin_amdgcn_readfirstlane(run_chunk(last, chunk, a.grain));
             it.u = run_at(a.c, a.R, it.run);
             it.ok = true;
             return it;

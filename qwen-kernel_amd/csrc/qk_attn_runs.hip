@@ -17,11 +17,12 @@ __global__ __launch_bounds__(256) void attn_join_kernel(RunsCall a)
     constexpr uint32_t PER = DH / 64; // floats per lane
     typedef float vec __attribute__((ext_vector_type(PER)));
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row = blockIdx.x;
-    const uint32_t chunk = *a.chunk_used;
+    const uint32_t common = *a.chunk_used;
     const uint32_t ri = wave_last_le(a.R.n_run, row, [&](uint32_t i) { return (int64_t)a.R.start[i]; });
     if (ri >= a.R.n_run) return; // the whole workgroup
     const Run u = run_at(a.c, a.R, ri);
     if (!u.ok || row - u.r0 >= u.n) return; // the whole workgroup
+    const uint32_t chunk = run_chunk(min(u.pos + u.n, a.c.cap), common, a.grain);
     const uint32_t n = __builtin_amdgcn_readfirstlane((min(u.pos + (row - u.r0) + 1, a.c.cap) + chunk - 1) / chunk);
     {
         const uint32_t h0 = blockIdx.y * 4 * HB + wave; // and every fourth behind it
@@ -81,7 +82,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(RunsCall a)
 // follows them): which kernel, and how short the ranges of keys that run in parallel may get.  The workspace is sized by it.
 struct Plan {
     bool few;
-    uint32_t n_split, chunk, slots;
+    uint32_t n_split, chunk, grain, slots;
 };
 static Plan plan_of(const qkk_kv_cache* C, const qkk_kv_runs* R, uint32_t hQ)
 {
@@ -98,9 +99,9 @@ static Plan plan_of(const qkk_kv_cache* C, const qkk_kv_runs* R, uint32_t hQ)
         const uint64_t groups = std::max<uint64_t>(((uint64_t)R->n_rows * G + AR_TILE_ROWS - 1) / AR_TILE_ROWS, R->n_run) * C->n_kv;
         ranges = groups >= 256 ? 1 : std::min<uint64_t>(64, (1024 + groups - 1) / groups);
     }
-    // a range is at least one step per wave (128 keys; 256 for few rows on halves with dh 128)
-    const uint64_t step = p.few && C->type == QKK_F16 && C->dh == 128 ? 256 : 128;
-    p.chunk = (uint32_t)std::max<uint64_t>(step, ((cap + ranges - 1) / ranges + step - 1) / step * step);
+    // few rows: a range is at least one step per wave (128 keys; 256 on halves with dh 128); many rows: one or two tiles
+    p.grain = !p.few ? 64 : C->type == QKK_F16 && C->dh == 128 ? 256 : 128;
+    p.chunk = (uint32_t)std::max<uint64_t>(1, ((cap + ranges - 1) / ranges + p.grain - 1) / p.grain) * p.grain;
     p.n_split = (uint32_t)((cap + p.chunk - 1) / p.chunk);
     return p;
 }
@@ -139,6 +140,7 @@ static int attn_runs(const char* who, const qkk_kv_cache* C, uint32_t layer, con
         a.G = hQ / c.n_kv;
         a.n_split = plan.n_split;
         a.chunk = plan.chunk;
+        a.grain = plan.grain;
         a.slots = plan.slots;
         a.chunk_used = (uint32_t*)(a.ml + 2 * (size_t)runs.n_rows * hQ * plan.n_split);
         if (plan.few) launch_attn_few(a, C->type, C->dh, tree, as_stream(stream));

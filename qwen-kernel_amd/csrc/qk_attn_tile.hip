@@ -119,7 +119,6 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
         f0 = (blk - (uint32_t)first_of(run)) * TL_M;
     } else {
         const Item it = item_of(a, blockIdx.x / a.c.n_kv, TL_M);
-        if (blockIdx.x == 0 && threadIdx.x == 0) *a.chunk_used = it.chunk;
         if (!it.ok) return; // the whole workgroup
         u = it.u;
         run = it.run;
@@ -137,48 +136,8 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
     const uint32_t node0 = f0 / a.G;
     if (TREE && k_end > u.pos) tree_bits(tree_parent(a.parent, u), node0, last - node0 + 1, s_up, s_kin);
 
-    // Q: this wave's rows f0 + WR wave + 16 rt + m, dims 32 ks + 8 g .. + 7, divided by the row's power of two
-    half8 qh[RT][KS], ql[RT][KS];
-    float q_fac[RT];
     const uint32_t wr = WR * wave; // the wave's first row in the block
     const bool has = wr < nr;      // uniform: a wave without rows only stages tiles
-#pragma unroll
-    for (uint32_t rt = 0; rt < RT; rt++) {
-        const uint32_t f = wr + 16 * rt + m, ff = f0 + min(f, nr - 1);
-        const f32x4* row = (const f32x4*)(a.q + ((size_t)(u.r0 + ff / a.G) * a.hQ + kv * a.G + ff % a.G) * DH);
-        f32x4 x[KS][2];
-        float mx = 0.f;
-#pragma unroll
-        for (uint32_t ks = 0; ks < KS; ks++)
-#pragma unroll
-            for (uint32_t i = 0; i < 2; i++) {
-                x[ks][i] = row[8 * ks + 2 * g + i];
-#pragma unroll
-                for (uint32_t j = 0; j < 4; j++) mx = fmaxf(mx, fabsf(x[ks][i][j]));
-            }
-        const int e = top_exponent(xor_lanes_max(mx));
-        const float scale = pow2i(-e);
-        q_fac[rt] = pow2i(e) * (AR_LOG2E / sqrtf((float)DH));
-#pragma unroll
-        for (uint32_t ks = 0; ks < KS; ks++) {
-            float y[8];
-#pragma unroll
-            for (uint32_t j = 0; j < 8; j++) y[j] = x[ks][j / 4][j % 4] * scale;
-            const Half2 sp = split2(y);
-            qh[rt][ks] = sp.hi;
-            ql[rt][ks] = sp.lo;
-        }
-    }
-    float4v o[RT][NT];
-    float m_run[RT], l_run[RT];
-#pragma unroll
-    for (uint32_t rt = 0; rt < RT; rt++) {
-        m_run[rt] = AR_FLOOR;
-        l_run[rt] = 0.f;
-#pragma unroll
-        for (uint32_t t = 0; t < NT; t++) o[rt][t] = float4v{0.f, 0.f, 0.f, 0.f};
-    }
-
     // this lane's rows' positions behind node0 (below 128), 255 for a row that is not there: a byte for each block, so one register
     uint32_t nodes = 0;
 #pragma unroll
@@ -353,6 +312,55 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
         }
         if (piece == 0) s_flag[sg * NB + st] = odd | bad_pages << 8;
     };
+    // Q: this wave's rows f0 + WR wave + 16 rt + m, dims 32 ks + 8 g .. + 7, requested in front of the first tile's rows and prepared, divided
+    // by the row's power of two, while those arrive
+    pages(0);
+    half8 qh[RT][KS], ql[RT][KS];
+    float q_fac[RT];
+    f32x4 qx[RT][KS][2];
+#pragma unroll
+    for (uint32_t rt = 0; rt < RT; rt++) {
+        const uint32_t ff = f0 + min(wr + 16 * rt + m, nr - 1);
+        const f32x4* row = (const f32x4*)(a.q + ((size_t)(u.r0 + ff / a.G) * a.hQ + kv * a.G + ff % a.G) * DH);
+#pragma unroll
+        for (uint32_t ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (uint32_t i = 0; i < 2; i++) qx[rt][ks][i] = row[8 * ks + 2 * g + i];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    fetch(0);
+    if (n_tile > 1) pages(1);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (uint32_t rt = 0; rt < RT; rt++) {
+        float mx = 0.f;
+#pragma unroll
+        for (uint32_t ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(qx[rt][ks][j / 4][j % 4]));
+        const int e = top_exponent(xor_lanes_max(mx));
+        const float scale = pow2i(-e);
+        q_fac[rt] = pow2i(e) * (AR_LOG2E / sqrtf((float)DH));
+#pragma unroll
+        for (uint32_t ks = 0; ks < KS; ks++) {
+            float y[8];
+#pragma unroll
+            for (uint32_t j = 0; j < 8; j++) y[j] = qx[rt][ks][j / 4][j % 4] * scale;
+            const Half2 sp = split2(y);
+            qh[rt][ks] = sp.hi;
+            ql[rt][ks] = sp.lo;
+        }
+    }
+    float4v o[RT][NT];
+    float m_run[RT], l_run[RT];
+#pragma unroll
+    for (uint32_t rt = 0; rt < RT; rt++) {
+        m_run[rt] = AR_FLOOR;
+        l_run[rt] = 0.f;
+#pragma unroll
+        for (uint32_t t = 0; t < NT; t++) o[rt][t] = float4v{0.f, 0.f, 0.f, 0.f};
+    }
+
     // Scores, softmax and values of a tile's 32 keys from 32 sp for this wave.  whole: every row sees every key.
     auto work = [&](uint32_t tile, const uint8_t* buf, bool whole, uint32_t sp) {
         const uint8_t* s_k = buf;
@@ -481,9 +489,6 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
         }
     };
 
-    pages(0);
-    fetch(0);
-    if (n_tile > 1) pages(1);
     stage(0, s_dyn);
     if (n_tile > 1) fetch(1);
     if (n_tile > 2) pages(2);
