@@ -478,15 +478,9 @@ static void launch_few(const RunsCall& a, bool tree, hipStream_t st)
     constexpr uint32_t q_bytes = (F32 ? 3 : 2) * RT * (DH / 32) * 1024, o_bytes = 2 * RT * 16 * (DH + 4) * 4;
     constexpr uint32_t lds = q_bytes > o_bytes ? q_bytes : o_bytes;
     const dim3 grid(items_of(a.R.n_run, a.slots, a.n_split) * a.c.n_kv), block(256);
-    if (tree) {
-        static bool once = ((void)hipFuncSetAttribute((const void*)attn_few_kernel<DH, F32, RT, true>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), true);
-        (void)once;
-        hipLaunchKernelGGL((attn_few_kernel<DH, F32, RT, true>), grid, block, lds, st, a);
-    } else {
-        static bool once = ((void)hipFuncSetAttribute((const void*)attn_few_kernel<DH, F32, RT, false>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), true);
-        (void)once;
-        hipLaunchKernelGGL((attn_few_kernel<DH, F32, RT, false>), grid, block, lds, st, a);
-    }
+    static_assert(lds <= 65536, "more would have to be asked for (allow_lds)");
+    if (tree) hipLaunchKernelGGL((attn_few_kernel<DH, F32, RT, true>), grid, block, lds, st, a);
+    else hipLaunchKernelGGL((attn_few_kernel<DH, F32, RT, false>), grid, block, lds, st, a);
 }
 
 void launch_attn_few(const RunsCall& a, int type, uint32_t dh, bool tree, hipStream_t st)

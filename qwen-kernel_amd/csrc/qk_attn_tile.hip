@@ -572,8 +572,8 @@ static void launch_tile(const RunsCall& a, hipStream_t st)
 {
     constexpr uint32_t lds = 2 * TileGeom<DH, F32>::BUF;
     static_assert(lds <= 160 * 1024, "LDS");
-    static bool once = ((void)hipFuncSetAttribute((const void*)attn_tile_kernel<DH, F32, TREE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds), true);
-    (void)once;
+    static std::atomic<uint64_t> asked{0};
+    allow_lds((const void*)attn_tile_kernel<DH, F32, TREE>, lds, asked);
     hipLaunchKernelGGL((attn_tile_kernel<DH, F32, TREE>), dim3(items_of(tile_blocks(a.R.n_rows, a.R.n_run, a.G), a.slots, a.n_split) * a.c.n_kv), dim3(64 * TileGeom<DH, F32>::WAVES), lds, st, a);
 }
 

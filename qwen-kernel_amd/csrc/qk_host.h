@@ -4,6 +4,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <atomic>
+
 #include "../../include/qk_kernels.h"
 
 namespace qk {
@@ -41,6 +43,18 @@ struct Options {
 };
 Options& options();
 void apply_env_options(Options& v); // qk_open reads the environment again: switches set since the first use take effect for the engine it builds
+
+// Lets a kernel take `bytes` of dynamic LDS (more than 64 KB have to be asked for), once per device: `done` is the kernel's own
+// record of the devices it has been asked for on.
+inline void allow_lds(const void* kernel, size_t bytes, std::atomic<uint64_t>& done)
+{
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev > 63) dev = 63;
+    const uint64_t bit = 1ull << dev;
+    if (dev < 63 && (done.load(std::memory_order_relaxed) & bit)) return;
+    (void)hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    done.fetch_or(bit, std::memory_order_relaxed);
+}
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

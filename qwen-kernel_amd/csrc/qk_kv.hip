@@ -53,8 +53,9 @@ __global__ __launch_bounds__(1024) void kv_resize_kernel(KvView c, int32_t* tabl
                                                          const int32_t* __restrict__ len_new, int32_t* status, KvWs ws)
 {
     __shared__ uint32_t s_wave[KV_TPB / 64], s_n, s_bad;
+    __shared__ unsigned long long s_need;
     const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
-    if (t == 0) { s_n = 0; s_bad = 0; }
+    if (t == 0) { s_n = 0; s_bad = 0; s_need = 0; }
     __syncthreads();
     for (uint32_t s = t; s < c.n_seq; s += KV_TPB)
         if (len_new[s] >= 0 && (uint32_t)len_new[s] > c.cap) s_bad = 1;
@@ -87,7 +88,7 @@ __global__ __launch_bounds__(1024) void kv_resize_kernel(KvView c, int32_t* tabl
     publish_wait(); // the references are back where ref_load reads them
     __syncthreads();
     // what the growing sequences need, and whether they begin with a copy of a shared page
-    uint32_t needed = 0;
+    uint32_t needed = 0; // exact where it matters: while all of it is no more than there are pages
     for (uint32_t s0 = 0; s0 < c.n_seq; s0 += KV_TPB) {
         const uint32_t s = s0 + t;
         uint32_t need = 0;
@@ -102,12 +103,16 @@ __global__ __launch_bounds__(1024) void kv_resize_kernel(KvView c, int32_t* tabl
                 need = pages_for(now, c.shift) - pages_for(old, c.shift) + split;
             }
             ws.need[s] = 2 * need + split;
+            if (need) atomicAdd(&s_need, (unsigned long long)need);
         }
         uint32_t total;
         const uint32_t before = block_scan(need, s_wave, total);
         if (s < c.n_seq) ws.first[s] = needed + before;
         needed += total;
     }
+    __syncthreads();
+    const uint64_t all = s_need;
+    if (all > c.n_page) needed = 0xFFFFFFFFu; // cannot be met: only the free pages are counted below
     // the free pages, lowest first, as many as are needed
     uint32_t found = 0;
     for (uint32_t p0 = 0; p0 < c.n_page && found < needed; p0 += KV_TPB) {
@@ -120,7 +125,7 @@ __global__ __launch_bounds__(1024) void kv_resize_kernel(KvView c, int32_t* tabl
     }
     __syncthreads();
     if (found < needed) {
-        if (t == 0) { *status = (int32_t)(needed - found); *ws.n_copy = 0; }
+        if (t == 0) { *status = (int32_t)min(all - found, (uint64_t)0x7FFFFFFF); *ws.n_copy = 0; }
         return;
     }
     for (uint32_t s = wave; s < c.n_seq; s += KV_TPB / 64) {
@@ -392,7 +397,7 @@ int qkk_kv_compact(const qkk_kv_cache* C, const int32_t* seq, const int32_t* bas
     if (n > C->n_seq || max_path > QKK_TREE_MAX)
         return fail(QKK_ESHAPE, "qkk_kv_compact: %u paths (of %u sequences) of up to %u rows (at most %u)", n, C->n_seq, max_path, QKK_TREE_MAX);
     const uint64_t jobs = (uint64_t)n * C->n_layer * C->n_kv * 2;
-    if (jobs > (1ull << 32)) return fail(QKK_ESHAPE, "qkk_kv_compact: paths x layers x heads too large");
+    if (jobs > (1ull << 25)) return fail(QKK_ESHAPE, "qkk_kv_compact: paths x layers x heads too large");
     if (int rc = require_device()) return rc;
     if (!n || !max_path) return QKK_OK;
     const uint32_t row_pieces = C->dh * (C->type == QKK_F32 ? 4 : 2) / 16;
