@@ -38,7 +38,7 @@ __global__ __launch_bounds__(256, (DH == 128 && RT == 1 ? 2 : 1)) void attn_few_
     __shared__ uint32_t s_kin[TREE ? RT * 16 : 1][QKK_TREE_MAX / 32];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 15u, g = lane >> 4;
     const uint32_t kv = blockIdx.x % a.c.n_kv;
-    const Item it = item_of(a, blockIdx.x / a.c.n_kv, RT * 16);
+    const Item it = item_of(a, blockIdx.x / a.c.n_kv, RT * 16, false);
     if (!it.ok) return; // the whole workgroup
     const Run u = it.u;
     const uint32_t run = it.run, split = it.split;

@@ -44,52 +44,73 @@ struct Item {
     uint32_t run, block, split, chunk;
     bool ok;
 };
-// Sequences of a batch differ in length by orders of magnitude, and the lengths live on the device.  Every wave looks all of them
-// over (64 runs per round trip), takes the range that cuts the whole of them -- blocks of `rows` rows times keys -- into as
-// many items as there are places on the device, and finds its own item by a prefix sum; items without work come last and end
-// at once.  A run's own ranges are then made equal.  (With ranges fixed by the host three of four workgroups of sixteen ragged sequences had no work, and those that had
-// some waited behind them: 37 us.)  Every workgroup comes to the same result; the join finds the common range in the workspace.
 // The length of a run's ranges, all but the last: as many as `chunk` makes, of one length.
 __device__ __forceinline__ uint32_t run_chunk(uint32_t end, uint32_t chunk, uint32_t grain)
 {
     const uint32_t splits = max((end + chunk - 1) / chunk, 1u), each = (end + splits - 1) / splits;
     return max((each + grain - 1) / grain, 1u) * grain;
 }
-__device__ __forceinline__ Item item_of(const RunsCall& a, uint32_t item, uint32_t rows)
+// Sequences of a batch differ in length by orders of magnitude, and the lengths live on the device.  Every wave looks all of them
+// over (64 runs per round trip, about 2 us), takes the range that cuts the whole of them -- blocks of `rows` rows times keys --
+// into as many items as there are places on the device, and finds its own item by a prefix sum; items without work come last
+// and end at once.  A run's own ranges are then made equal.  Every workgroup comes to the same result; the join finds the common
+// range in the workspace.  (One row for each of sixteen sequences of 1 .. 4096 keys: 25 us, 37 with ranges fixed by the host, where three
+// workgroups of four had no work and the others waited behind them.)
+//   Packed rows see half of their own run on average: their work is counted so, and ranges that a block of rows does not reach
+// end at once.  A block's last range is half empty on average; where that guess makes more items than places, the range is taken
+// that cannot: a second round on the device costs more than shorter ranges give.  (Counting a whole range lost per block
+// left a tenth of the device idle: trees of 24 nodes on sixteen slots
+// of 1000 .. 4100 fp32 rows 129 us, 119 so; two trees on 33,000 and 65,000 half rows 204 and 198.)
+__device__ __forceinline__ Item item_of(const RunsCall& a, uint32_t item, uint32_t rows, bool causal)
 {
     const uint32_t lane = threadIdx.x & 63u;
-    auto look = [&](uint32_t i, uint32_t& nb, uint32_t& end) {
-        nb = end = 0;
+    auto look = [&](uint32_t i, uint32_t& nb, uint32_t& end, uint32_t& seen) {
+        nb = end = seen = 0;
         if (i >= a.R.n_run) return;
         const Run u = run_at(a.c, a.R, i);
         if (!u.ok || !u.n) return;
         nb = (u.n * a.G + rows - 1) / rows;
         end = min(u.pos + u.n, a.c.cap);
+        seen = causal ? min(u.pos + (u.n + 1) / 2, end) : end; // at least half of end
     };
-    uint32_t nb0, end0, blocks = 0; // the first 64 runs stay in registers
+    uint32_t nb0, end0, seen0, blocks = 0; // the first 64 runs stay in registers
     uint64_t work = 0;              // in pieces of 64 keys
-    look(lane, nb0, end0);
+    look(lane, nb0, end0, seen0);
     for (uint32_t i = lane; i < a.R.n_run; i += 64) {
-        uint32_t nb = nb0, end = end0;
-        if (i != lane) look(i, nb, end);
+        uint32_t nb = nb0, end = end0, seen = seen0;
+        if (i != lane) look(i, nb, end, seen);
         blocks += nb;
-        work += (uint64_t)nb * ((end + 63) / 64);
+        work += (uint64_t)nb * ((seen + 63) / 64);
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
         blocks += __shfl_xor(blocks, d);
         work += __shfl_xor(work, d);
     }
-    const uint64_t places = a.slots > 2 * blocks ? a.slots - blocks : max(blocks, 1u);
-    const uint64_t want = ((work + places - 1) / places * 64 + a.grain - 1) / a.grain * a.grain;
+    auto range_for = [&](uint32_t places) {
+        const uint64_t want = ((work + places - 1) / places * 64 + a.grain - 1) / a.grain * a.grain;
+        return (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)min(max(want, (uint64_t)a.chunk), (uint64_t)1 << 30));
+    };
+    const uint32_t least = max(a.slots / 2, 1u);
+    uint32_t chunk = range_for(max(a.slots - min(blocks / 2, a.slots), least));
+    if (!causal) {
+        uint32_t made = 0;
+        for (uint32_t i = lane; i < a.R.n_run; i += 64) {
+            uint32_t nb = nb0, end = end0, seen = seen0;
+            if (i != lane) look(i, nb, end, seen);
+            made += nb * ((end + chunk - 1) / chunk);
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) made += __shfl_xor(made, d);
+        if (made > a.slots) chunk = range_for(max(a.slots - min(blocks, a.slots), least)); // uniform
+    }
     Item it;
-    const uint32_t chunk = __builtin_amdgcn_readfirstlane((uint32_t)min(max(want, (uint64_t)a.chunk), (uint64_t)1 << 30));
     if (blockIdx.x == 0 && threadIdx.x == 0 && a.n_split > 1) *a.chunk_used = chunk;
     it.ok = false;
     uint32_t before = 0;
     for (uint32_t i0 = 0; i0 < a.R.n_run; i0 += 64) {
-        uint32_t nb = nb0, end = end0;
-        if (i0) look(i0 + lane, nb, end);
+        uint32_t nb = nb0, end = end0, seen = seen0;
+        if (i0) look(i0 + lane, nb, end, seen);
         const uint32_t mine = nb * ((end + chunk - 1) / chunk), incl = before + wave_incl_scan_u32(mine);
         const uint64_t past = __builtin_amdgcn_ballot_w64(incl > item);
         if (past) {
@@ -250,11 +271,12 @@ __device__ __forceinline__ uint32_t tree_four(const uint32_t* kin, int32_t rel)
 constexpr uint32_t AR_TILE_ROWS = 128;
 inline uint32_t tile_blocks(uint32_t n_rows, uint32_t n_run, uint32_t G) { return (uint32_t)((uint64_t)n_rows * G / AR_TILE_ROWS) + n_run; }
 
-// Items of one KV head that a launch has to have room for, `blocks` the blocks of rows at most (item_of makes no more than `slots` of
-// them, or two per block): one per block where the keys are not cut.
+// Items of one KV head that a launch has to have room for, `blocks` the blocks of rows at most.  item_of cuts what is seen, at least half
+// of what it counts out, into no more than `slots` full ranges, and every block may have one that is not full.  One per block where
+// the keys are not cut.
 inline uint32_t items_of(uint32_t blocks, uint32_t slots, uint32_t n_split)
 {
-    const uint64_t all = (uint64_t)blocks * n_split, made = slots > 2 * blocks ? slots : 2ull * blocks;
+    const uint64_t all = (uint64_t)blocks * n_split, made = 2ull * slots + blocks;
     return (uint32_t)(n_split == 1 ? blocks : all < made ? all : made);
 }
 

@@ -124,7 +124,7 @@ static int attn_runs(const char* who, const qkk_kv_cache* C, uint32_t layer, con
     if (int rc = require_device()) return rc;
     if (!runs.n_rows || !runs.n_run) return QKK_OK;
     const Plan plan = plan_of(C, R, hQ);
-    if (2 * (uint64_t)(tile_blocks(runs.n_rows, runs.n_run, hQ / c.n_kv)) * c.n_kv > (1u << 22) || (uint64_t)runs.n_rows * hQ > (1u << 30))
+    if (((uint64_t)(tile_blocks(runs.n_rows, runs.n_run, hQ / c.n_kv)) + 2 * plan.slots) * c.n_kv > (1u << 22) || (uint64_t)runs.n_rows * hQ > (1u << 30))
         return fail(QKK_ESHAPE, "%s: rows x heads or runs x heads too large", who);
     {
         RunsCall a;

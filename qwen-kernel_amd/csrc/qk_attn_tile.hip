@@ -118,7 +118,7 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
         u = run_at(a.c, a.R, run);
         f0 = (blk - (uint32_t)first_of(run)) * TL_M;
     } else {
-        const Item it = item_of(a, blockIdx.x / a.c.n_kv, TL_M);
+        const Item it = item_of(a, blockIdx.x / a.c.n_kv, TL_M, !TREE);
         if (!it.ok) return; // the whole workgroup
         u = it.u;
         run = it.run;
