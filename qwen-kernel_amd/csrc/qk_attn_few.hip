@@ -15,6 +15,8 @@
 // An fp32 cache is split into three bf16 pieces in registers (exact, fp32's whole range, NaN and infinities stay in their
 // key), six of the nine products are kept (the others are below 2^-23 of their terms); a half cache is an operand as it is,
 // and queries and weights go in as hi + lo halves: two products.  Matrix work is a few percent of the time either way.
+//   One row for each of sixteen sequences of 1 .. 4096 half rows, 32 heads on 8 of 128 (63 MB): 21 us and 4 us for the join, 2.6 TB/s
+// where a large copy moves 4.8; six of the 21 pass before the first keys arrive (lengths, page ids, keys: three round trips).
 #include "qk_attn_runs.h"
 
 namespace qk {

@@ -54,13 +54,13 @@ __device__ __forceinline__ uint32_t run_chunk(uint32_t end, uint32_t chunk, uint
 // over (64 runs per round trip, about 2 us), takes the range that cuts the whole of them -- blocks of `rows` rows times keys --
 // into as many items as there are places on the device, and finds its own item by a prefix sum; items without work come last
 // and end at once.  A run's own ranges are then made equal.  Every workgroup comes to the same result; the join finds the common
-// range in the workspace.  (One row for each of sixteen sequences of 1 .. 4096 keys: 25 us, 37 with ranges fixed by the host, where three
-// workgroups of four had no work and the others waited behind them.)
+// range in the workspace.  (One row for each of sixteen sequences of 1 .. 4096 keys: 25 us, 37 with ranges fixed by the host,
+// where three workgroups of four had no work and the others waited behind them.)
 //   Packed rows see half of their own run on average: their work is counted so, and ranges that a block of rows does not reach
 // end at once.  A block's last range is half empty on average; where that guess makes more items than places, the range is taken
 // that cannot: a second round on the device costs more than shorter ranges give.  (Counting a whole range lost per block
-// left a tenth of the device idle: trees of 24 nodes on sixteen slots
-// of 1000 .. 4100 fp32 rows 129 us, 119 so; two trees on 33,000 and 65,000 half rows 204 and 198.)
+// left a tenth of the device idle: trees of 24 nodes on sixteen slots of 1000 .. 4100 fp32 rows 129 us, 119 so; two trees on
+// 33,000 and 65,000 half rows 204 and 198.)
 __device__ __forceinline__ Item item_of(const RunsCall& a, uint32_t item, uint32_t rows, bool causal)
 {
     const uint32_t lane = threadIdx.x & 63u;

@@ -9,8 +9,9 @@
 namespace qk {
 
 // One workgroup per row and 4 HB heads: folds their ranges in range order and applies the gate, each wave HB heads side by side.  Ranges
-// behind the row's own position hold nothing for it.  A chain of round trips: HB = 4 where that still fills the device (763 rows of
-// 16 heads: 15.4 -> 11 us), one head per wave where there are few rows (16 of 32 heads: 4.6 us against 9).
+// behind the row's own position hold nothing for it.  A chain of round trips (run -> sums -> ranges),
+// 5 to 13 us where its bytes would take 1 to 4: HB = 4 where that still fills the device (763 rows of 16 heads: 12.4 us, 15.7
+// with one head per wave), one head per wave where there are few rows (16 of 32 heads: 3.9 us against 9).
 template <int DH, int HB>
 __global__ __launch_bounds__(256) void attn_join_kernel(RunsCall a)
 {

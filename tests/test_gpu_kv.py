@@ -52,6 +52,30 @@ def test_serving_sequence(qk, up, ws, dev, type_, dh, hq, hkv, page):
     KC.serve_case(qk, up, ws, type_, dh, hq, hkv, page, sync=torch.cuda.synchronize)
 
 
+def test_same_cache_as_the_slot_kernels(qk, dev, ws):
+    """The slot kernels' caches are a slot cache of one layer: a tree of one node is qkk_attn_decode's step, a packed prompt
+    qkk_attn_seq's.  1e-5 of the largest value is what the slot kernels' own forms are held to between each other."""
+    import torch
+    g = torch.Generator(dev).manual_seed(5)
+    rnd = lambda *s: torch.randn(*s, generator=g, device=dev)  # noqa: E731
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    k, v = rnd(3, 2, 700, 256), rnd(3, 2, 700, 256)
+    cache = qk.KvCache(k[None], v[None])
+    q, qfull, at = rnd(3, 16, 256), rnd(3, 16, 512), (699, 0, 130)
+    runs = qk.KvRuns(3, i32(0, 1, 2, 3), i32(0, 1, 2), i32(*at), max_run=1)
+    room = [ws(b).zero_() for b in (qk.attn_runs_workspace_bytes(cache, runs, 16), qk.attn_workspace_bytes(64, 16))]
+    mine = qk.attn_tree(cache, 0, runs, i32(-1, -1, -1), q, room[0], qfull=qfull)
+    theirs = qk.attn_decode(q, k, v, qfull, i32(*at), room[1])
+    assert (mine - theirs).abs().max() <= 1e-5 * theirs.abs().max()
+    n, base = 60, 333
+    q, qfull = rnd(n, 16, 256), rnd(n, 16, 512)
+    runs = qk.KvRuns(n, i32(0, n), i32(2), i32(base))
+    room = [ws(b).zero_() for b in (qk.attn_runs_workspace_bytes(cache, runs, 16), qk.attn_workspace_bytes(64, 16))]
+    mine = qk.attn_packed(cache, 0, runs, q, room[0], qfull=qfull)
+    theirs = qk.attn_decode(q, k[2:], v[2:], qfull, torch.arange(base, base + n, dtype=torch.int32, device=dev), room[1], seq=True)
+    assert (mine - theirs).abs().max() <= 1e-5 * theirs.abs().max()
+
+
 # ---- larger sizes, against the definition in 64 bits on the device -----------------------------------------------------
 
 def exact(cache, layer, runs, lens, past, q, gate, parent):
