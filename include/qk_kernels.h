@@ -426,7 +426,9 @@ int qkk_dn_step_seq(const float *conv, const float *gb, float *state, const floa
  * start[i] .. start[i+1]-1 (ascending, start[n_run] <= n_rows; empty runs are allowed; rows in no run are
  * left as they were), belongs to sequence seq[i], and its first row is cache row pos[i].  No run is longer
  * than max_run (rows behind that are left as they were): it chooses the launch shape.  start, seq and pos
- * are DEVICE arrays, so a captured graph follows them.  A run with seq or pos out of range is left out. */
+ * are DEVICE arrays, so a captured graph follows them.  A run with seq or pos out of range is left out.  Runs
+ * that write the same cache rows in one call race for them.  Without rows or runs a call does nothing, and
+ * arrays without elements may be NULL. */
 typedef struct qkk_kv_cache {
     int32_t type;
     uint32_t n_layer, n_page, n_kv, page_rows, dh, n_seq, seq_pages;
@@ -500,8 +502,8 @@ int qkk_attn_tree(const qkk_kv_cache *C_host, uint32_t layer, const qkk_kv_runs 
  * qkk_kv_compact for i < n: of the drafted rows behind cache row base[i] of sequence seq[i], row
  *                base + path[i][j] is moved to base + j, j < n_path[i] (path [n][max_path], ascending):
  *                the accepted path of a tree to the front.  A path that is not strictly ascending, or
- *                leaves the sequence's pages, is left out (nothing of it is moved).  Touches no books; each
- *                sequence once.  max_path <= QKK_TREE_MAX. */
+ *                leaves the sequence's pages, is left out (nothing of it is moved).  Touches no books.  A
+ *                sequence comes once per call (two paths of one race for its rows).  max_path <= QKK_TREE_MAX. */
 size_t qkk_kv_workspace_bytes(const qkk_kv_cache *C_host);
 int qkk_kv_resize(const qkk_kv_cache *C_host, const int32_t *len_new, int32_t *status, void *workspace,
                   size_t workspace_bytes, void *stream);

@@ -127,7 +127,7 @@ int qkk_attn_prep_axes(const qkk_kv_cache* C, uint32_t layer, const qkk_kv_runs*
     RunsView runs;
     if (int rc = kv_view(who, C, layer, &c)) return rc;
     if (int rc = runs_view(who, R, &runs)) return rc;
-    if (!q || !kin || !vin || !q_norm_w || !k_norm_w || !rope || !pair_axis || !axis_pos || !qhat) return fail(QKK_EINVAL, "%s: null pointer", who);
+    if (!q_norm_w || !k_norm_w || !rope || !pair_axis || (runs.n_rows && (!q || !kin || !vin || !axis_pos || !qhat))) return fail(QKK_EINVAL, "%s: null pointer", who);
     if (!aligned16(q) || !aligned16(kin) || !aligned16(vin) || !aligned16(qhat) || !aligned16(q_norm_w) || !aligned16(k_norm_w) || !aligned16(rope))
         return fail(QKK_EINVAL, "%s: q, kin, vin, qhat, the norm weights and rope must be 16-byte aligned", who);
     if (hQ < 1 || hQ > 4096) return fail(QKK_ESHAPE, "%s: %u query heads outside 1..4096", who, hQ);

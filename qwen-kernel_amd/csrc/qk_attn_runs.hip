@@ -114,7 +114,7 @@ static int attn_runs(const char* who, const qkk_kv_cache* C, uint32_t layer, con
     RunsView runs;
     if (int rc = kv_view(who, C, layer, &c)) return rc;
     if (int rc = runs_view(who, R, &runs)) return rc;
-    if (!qhat || !att || !workspace || (tree && !parent)) return fail(QKK_EINVAL, "%s: null pointer", who);
+    if (!workspace || (runs.n_rows && (!qhat || !att || (tree && !parent)))) return fail(QKK_EINVAL, "%s: null pointer", who);
     if (hQ < c.n_kv || hQ % c.n_kv || hQ > 4096)
         return fail(QKK_ESHAPE, "%s: %u query heads on %u KV heads not supported (a multiple, at most 4096)", who, hQ, c.n_kv);
     if (tree && runs.max_run > QKK_TREE_MAX) return fail(QKK_ESHAPE, "%s: trees of up to %u nodes (at most %u)", who, runs.max_run, QKK_TREE_MAX);

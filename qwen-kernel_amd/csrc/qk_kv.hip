@@ -325,7 +325,7 @@ int kv_view(const char* who, const qkk_kv_cache* C, uint32_t layer, KvView* view
 
 int runs_view(const char* who, const qkk_kv_runs* R, RunsView* view)
 {
-    if (!R || !R->start || !R->seq || !R->pos) return fail(QKK_EINVAL, "%s: null pointer", who);
+    if (!R || (R->n_run && (!R->start || !R->seq || !R->pos))) return fail(QKK_EINVAL, "%s: null pointer", who);
     if (R->n_rows > (1u << 20) || R->n_run > (1u << 20)) return fail(QKK_ESHAPE, "%s: more than 2^20 rows or runs", who);
     *view = RunsView{R->start, R->seq, R->pos, R->n_rows, R->n_run, std::min(R->max_run, R->n_rows)};
     return QKK_OK;
@@ -395,7 +395,7 @@ int qkk_kv_compact(const qkk_kv_cache* C, const int32_t* seq, const int32_t* bas
 {
     KvView view;
     if (int rc = kv_view("qkk_kv_compact", C, 0, &view)) return rc;
-    if (n && (!seq || !base || !path || !n_path)) return fail(QKK_EINVAL, "qkk_kv_compact: null pointer");
+    if (n && max_path && (!seq || !base || !path || !n_path)) return fail(QKK_EINVAL, "qkk_kv_compact: null pointer");
     if (n > C->n_seq || max_path > QKK_TREE_MAX)
         return fail(QKK_ESHAPE, "qkk_kv_compact: %u paths (of %u sequences) of up to %u rows (at most %u)", n, C->n_seq, max_path, QKK_TREE_MAX);
     const uint64_t jobs = (uint64_t)n * C->n_layer * C->n_kv * 2;

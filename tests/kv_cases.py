@@ -451,3 +451,26 @@ ODD = [
 ]
 # scores forty times as large: a score's error, and with it a weight's, grows with them
 ODD_L2 = {"peaked": 40 * 4e-6, "peaked, half": 40 * 4e-6}
+
+
+def nothing_case(qk, up, ws):
+    """Calls without rows, runs, forks or paths do nothing, though their empty tensors have no address."""
+    rng = np.random.default_rng(3)
+    c = make_cache(rng, "f32", 1, 2, 128, 16, 64, (20, 0))
+    cache = device_cache(qk, up, c)
+    i32 = lambda *s: up(np.zeros(s, np.int32))  # noqa: E731
+    f32 = lambda *s: up(np.zeros(s, np.float32))  # noqa: E731
+    room = ws(max(qk.kv_workspace_bytes(cache), 4096))
+    for n_rows, n_run in ((0, 0), (0, 1), (3, 0)):
+        runs = qk.KvRuns(n_rows, i32(n_run + 1), i32(n_run), i32(n_run))
+        q, kv = f32(n_rows, 4, 128), f32(n_rows, 2, 128)
+        qhat, att = up(np.full((n_rows, 4, 128), 7, np.float32)), up(np.full((n_rows, 4, 128), 7, np.float32))
+        qk.attn_prep_axes(cache, 0, runs, q, kv, kv, f32(128), f32(128), f32(64, 32, 2), up(np.zeros(32, np.uint8)), i32(1, n_rows), qhat=qhat)
+        qk.attn_packed(cache, 0, runs, q, room, att=att)
+        qk.attn_tree(cache, 0, runs, i32(n_rows), q, room, att=att)
+        assert (host(qhat) == 7).all() and (host(att) == 7).all()
+    assert host(qk.kv_fork(cache, i32(0), i32(0), room)).tolist() == [0]
+    qk.kv_compact(cache, i32(0), i32(0), i32(0, 4), i32(0))
+    qk.kv_compact(cache, i32(1), i32(1), i32(1, 0), i32(1))
+    assert same(host(cache.k), c["k"]) and same(host(cache.v), c["v"])
+    assert same(host(cache.table), c["table"]) and same(host(cache.ref), c["ref"]) and same(host(cache.len), c["len"])

@@ -52,6 +52,10 @@ def test_serving_sequence(qk, up, ws, dev, type_, dh, hq, hkv, page):
     KC.serve_case(qk, up, ws, type_, dh, hq, hkv, page, sync=torch.cuda.synchronize)
 
 
+def test_calls_without_work(qk, up, ws):
+    KC.nothing_case(qk, up, ws)
+
+
 def test_same_cache_as_the_slot_kernels(qk, dev, ws):
     """The slot kernels' caches are a slot cache of one layer: a tree of one node is qkk_attn_decode's step, a packed prompt
     qkk_attn_seq's.  1e-5 of the largest value is what the slot kernels' own forms are held to between each other."""

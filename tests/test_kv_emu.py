@@ -39,6 +39,10 @@ def test_serving_sequence(qk, emu, type_, dh, hq, hkv, page):
     KC.serve_case(qk, emu.tensor, emu.workspace, type_, dh, hq, hkv, page)
 
 
+def test_calls_without_work(qk, emu):
+    KC.nothing_case(qk, emu.tensor, emu.workspace)
+
+
 def test_results_do_not_depend_on_the_order_of_the_threads(qk, emu):
     """The same bits whatever order the threads of a workgroup run in between two barriers (a missing barrier shows)."""
     L = emu_util.emu_lib(qk)
