@@ -14,7 +14,8 @@
 //   F16 cache   K and V are operands as they are, Q and P are hi + lo halves: two products.
 //   F32 cache   every row of K and V is divided by the power of two that brings its largest value into [1, 2) and split
 //               into hi + lo halves, three products (lo . lo is below 2^-22 of its term).  The powers of two go back in where they
-//               cost nothing: a key's into the factor of its scores, a value row's into the exponent of its weight -- P V = (P 2^e)
+//               cost nothing: a key's and a query's, added, into their scores (a product of both as factors would pass fp32's range
+//               where the score does not), a value row's into the exponent of its weight -- P V = (P 2^e)
 //               (V 2^-e), so the running maximum is kept over score + e -- and out of the sum again.  So fp32's range holds,
 //               row by row, with half the matrix work of three bf16 pieces.
 // Weights are kept around 2^6 rather than 1, which keeps the lo halves of small ones normal; the sum has the same factor.
@@ -30,6 +31,8 @@ namespace qk {
 typedef u32x4 __attribute__((may_alias)) lds_u32x4;
 typedef u32x2 __attribute__((may_alias)) lds_u32x2;
 typedef f32x4 __attribute__((may_alias)) lds_f32x4;
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+typedef i32x4 __attribute__((may_alias)) lds_i32x4;
 
 constexpr uint32_t TL_M = AR_TILE_ROWS;
 // The running maximum is moved only when a score passes it by more than 2^TL_SLACK: weights stay below 2^(TL_UP + TL_SLACK), inside a
@@ -47,7 +50,7 @@ struct TileGeom {
     static constexpr uint32_t KB = BN * DH * 2, VB = KB;           // bytes of one copy of K, of V^T
     static constexpr uint32_t RL = F32 ? 8 : 16, QL = 64 / RL;     // staging K: rows, and pieces of each, per wave and load
     static constexpr uint32_t PI = LPR / QL, KR = 8 / PI;          // loads per row, rows per thread
-    static constexpr uint32_t EXP = F32 ? 3 * BN * 4 : 0;          // per key: factor of the score, exponent and factor of the value row
+    static constexpr uint32_t EXP = F32 ? 3 * BN * 4 : 0;          // per key: exponent of the score, exponent and factor of the value row
     static constexpr uint32_t BUF = NH * (KB + VB) + EXP + 64;     // + flags [4 NB]
     // Operand fragments read ahead of the products, and whether that order is pinned: left to itself the scheduler keeps two in flight,
     // which costs dh 256 4 % and suits halves with dh 128; fp32 with dh 128 has registers for one only.
@@ -220,7 +223,7 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
                     mx = xor_lanes_max(mx);
                     const int ex = top_exponent(mx);
                     const float scale = pow2i(-ex);
-                    if (kq == 0) s_e[row] = pow2i(ex);
+                    if (kq == 0) s_e[row] = u2f((uint32_t)ex);
                     at += kq / 2 * 256 + kq % 2 * 8;
 #pragma unroll
                     for (uint32_t i = 0; i < T::PI; i++) { // pieces kq + 8 i: step i of 32 dims
@@ -320,8 +323,10 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
     // Q: this wave's rows f0 + WR wave + 16 rt + m, dims 32 ks + 8 g .. + 7, requested in front of the first tile's rows and prepared, divided
     // by the row's power of two, while those arrive
     pages(0);
+    // (and multiplied by log2 e / sqrt dh: scores are in the log2 domain)
     half8 qh[RT][KS], ql[RT][KS];
-    float q_fac[RT];
+    int q_exp[RT];
+    const float qs = AR_LOG2E / sqrtf((float)DH);
     f32x4 qx[RT][KS][2];
 #pragma unroll
     for (uint32_t rt = 0; rt < RT; rt++) {
@@ -343,14 +348,13 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
         for (uint32_t ks = 0; ks < KS; ks++)
 #pragma unroll
             for (uint32_t j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(qx[rt][ks][j / 4][j % 4]));
-        const int e = top_exponent(xor_lanes_max(mx));
-        const float scale = pow2i(-e);
-        q_fac[rt] = pow2i(e) * (AR_LOG2E / sqrtf((float)DH));
+        q_exp[rt] = top_exponent(xor_lanes_max(mx) * qs);
+        const float scale = pow2i(-q_exp[rt]);
 #pragma unroll
         for (uint32_t ks = 0; ks < KS; ks++) {
             float y[8];
 #pragma unroll
-            for (uint32_t j = 0; j < 8; j++) y[j] = qx[rt][ks][j / 4][j % 4] * scale;
+            for (uint32_t j = 0; j < 8; j++) y[j] = qx[rt][ks][j / 4][j % 4] * qs * scale;
             const Half2 sp = split2(y);
             qh[rt][ks] = sp.hi;
             ql[rt][ks] = sp.lo;
@@ -408,18 +412,19 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
         // scores in the log2 domain: this lane's row wr + 16 rt + m, keys 16 b + 4 g + r
 #pragma unroll
         for (uint32_t b = 0; b < 2; b++) {
-            f32x4 kf, ve;
+            i32x4 ke;
+            f32x4 ve;
             if constexpr (F32) {
                 const uint32_t j = 32 * sp + 16 * b + 4 * g;
-                kf = *(const lds_f32x4*)(s_e + j);
+                ke = *(const lds_i32x4*)(s_e + j);
                 ve = *(const lds_f32x4*)(s_e + BN + j);
             }
 #pragma unroll
             for (uint32_t r = 0; r < 4; r++) {
 #pragma unroll
                 for (uint32_t rt = 0; rt < RT; rt++) {
-                    if constexpr (F32) s[rt][b][r] = s[rt][b][r] * (kf[r] * q_fac[rt]) + ve[r];
-                    else s[rt][b][r] *= q_fac[rt];
+                    if constexpr (F32) s[rt][b][r] = __builtin_ldexpf(s[rt][b][r], ke[r] + q_exp[rt]) + ve[r];
+                    else s[rt][b][r] = __builtin_ldexpf(s[rt][b][r], q_exp[rt]);
                 }
             }
         }

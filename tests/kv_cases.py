@@ -474,3 +474,59 @@ def nothing_case(qk, up, ws):
     qk.kv_compact(cache, i32(1), i32(1), i32(1, 0), i32(1))
     assert same(host(cache.k), c["k"]) and same(host(cache.v), c["v"])
     assert same(host(cache.table), c["table"]) and same(host(cache.ref), c["ref"]) and same(host(cache.len), c["len"])
+
+
+# ---- the range of values -----------------------------------------------------------------------------------------------
+
+def check_range(got, want, rows, per, tol=4e-6):
+    """Relative error (2-norm) of every row's heads ("row") or of every dim over all rows ("dim"): what one large row, or one large dim,
+    would hide in the whole result.  The tolerance is that of the whole result at the head of this file, a bound of each element's
+    own rounding errors taken for signs at random: a row's 128 or 256 elements and a dim's rows and heads are as many."""
+    live = sorted({r for r, *_ in rows})
+    a, b = got[live].astype(np.float64), want[live]
+    assert np.isfinite(a).all()
+    axis = 2 if per == "row" else (0, 1)
+    off, size = np.sqrt(((a - b) ** 2).sum(axis)), np.sqrt((b ** 2).sum(axis))
+    worst = (off / np.where(size > 0, size, 1)).max()
+    assert worst <= tol, (per, worst)
+
+
+def range_case(qk, up, ws, case, edit, per, seed=0, tol=4e-6):
+    """One call whose values, keys or queries `edit` spreads over fp32's range, held to every row's or dim's own size."""
+    box = {}
+
+    def both(x):
+        edit(x)
+        box.update(x)
+    got, want = att_case(qk, up, ws, case, seed=seed, poison=False, edit=both, l2=np.inf)
+    rows = list(OK.runs(got.shape[0], box["start"], box["seq"], box["pos"], oracle_cache(box["c"]), box["max_run"]))
+    check_range(got, want, rows, per, tol)
+
+
+# many rows (several ranges of keys, one range, a tree) and few rows
+FORMS = [("many rows", ("f32", 256, 4, 2, 16, 160, (20, 9), (90, 65), False, 0)), ("many rows, one range", ("f32", 128, 8, 1, 0, 64, (20, 9), (43, 40), True, 0)),
+         ("wide tree", ("f32", 128, 8, 2, 16, 192, (20, 9), (120, 65), False, 2)), ("few rows", ("f32", 256, 4, 2, 16, 160, (5, 1), (140, 65), False, 2))]
+
+
+def _far_and_apart(p):
+    """Keys and queries of size 2^p that share no dim: every score is zero though the product of their sizes passes fp32's range."""
+    def edit(x):
+        half = x["q"].shape[2] // 2
+        x["c"]["k"] *= np.float32(2.0 ** p)
+        x["c"]["k"][..., :half] = 0
+        x["q"] *= np.float32(2.0 ** p)
+        x["q"][..., half:] = 0
+    return edit
+
+
+def _sizes_cancel(p):
+    """Keys of size 2^p, queries of size 2^-p: ordinary scores."""
+    def edit(x):
+        x["c"]["k"] *= np.float32(2.0 ** p)
+        x["q"] *= np.float32(2.0 ** -p)
+    return edit
+
+
+RANGE_SCORE = [(f"{what}, {where}", case, edit) for what, edit in [("keys and queries of size 2^70 in dims of their own", _far_and_apart(70)),
+                                                                  ("keys 2^100, queries 2^-100", _sizes_cancel(100)), ("keys 2^-100, queries 2^100", _sizes_cancel(-100))]
+               for where, case in FORMS]

@@ -277,3 +277,10 @@ def test_side_stream(qk, dev, up, ws):
         got = qk.attn_packed(cache, 0, runs, late, space)
     side.synchronize()
     assert torch.equal(got, want)
+
+
+# ---- the range of values -----------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("name,case,edit", KC.RANGE_SCORE, ids=[c[0] for c in KC.RANGE_SCORE])
+def test_scores_of_far_keys_and_queries(qk, up, ws, name, case, edit):
+    KC.range_case(qk, up, ws, case, edit, "row")

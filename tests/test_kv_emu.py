@@ -58,3 +58,8 @@ def test_results_do_not_depend_on_the_order_of_the_threads(qk, emu):
         L.emu_set_schedule(0, 0)
     for other in got[1:]:
         assert all(KC.same(a, b) for a, b in zip(got[0], other))
+
+
+@pytest.mark.parametrize("name,case,edit", KC.RANGE_SCORE, ids=[c[0] for c in KC.RANGE_SCORE])
+def test_scores_of_far_keys_and_queries(qk, emu, name, case, edit):
+    KC.range_case(qk, emu.tensor, emu.workspace, case, edit, "row")
