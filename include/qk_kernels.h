@@ -471,7 +471,8 @@ int qkk_attn_prep_axes(const qkk_kv_cache *C_host, uint32_t layer, const qkk_kv_
  *                  of one node is the decode step.
  * A row that sees nothing gives zeros.  What a row does not see never enters its result, whatever the
  * cache holds there; what it sees and is not finite makes it NaN or infinite (a score of minus infinity is a
- * weight of zero).  Value rows of an F32 cache that lie wholly below 2^-90 lose precision.
+ * weight of zero).  Value rows of an F32 cache may differ in size as far as fp32 reaches (below 2^-126 they
+ * may count as zeros).
  * The softmax's maximum and sum and all sums are fp32.  The same call gives the same bits.  Into how many
  * ranges the keys are cut, and with it the last bits of a row, depends on the lengths of all runs of the call.
  *   workspace: qkk_attn_runs_workspace_bytes(), 256-byte aligned, no initialisation needed; calls (and

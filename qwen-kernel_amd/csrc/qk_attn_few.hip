@@ -448,7 +448,7 @@ __global__ __launch_bounds__(256, (DH == 128 && RT == 1 ? 2 : 1)) void attn_few_
         const uint32_t f = 16 * rt + m;
         if (f >= nr) continue;
         const size_t rh = (size_t)(u.r0 + f / a.G) * a.hQ + kv * a.G + f % a.G;
-        const float inv = a.n_split > 1 ? UNIT : l_run[rt] == 0.f ? 0.f : UNIT / l_run[rt];
+        const float inv = l_run[rt] == 0.f ? 0.f : UNIT / l_run[rt];
         float* out = a.n_split > 1 ? a.acc + (rh * a.n_split + split) * DH : a.att + rh * DH;
         if (a.n_split > 1 && g == 0) {
             a.ml[2 * (rh * a.n_split + split)] = m_run[rt];

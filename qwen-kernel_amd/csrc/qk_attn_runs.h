@@ -26,14 +26,15 @@ constexpr float AR_FLOOR = -3.0e38f;
 constexpr float AR_LOG2E = 1.44269504088896341f;
 
 // One call.  With n_split 1 a workgroup takes all keys of its rows and writes att.  Else the keys are cut into ranges, each range's
-// (maximum, sum, weighted sum) go to the workspace and attn_join_kernel folds them.  How long a range is, is decided on the
+// result goes to the workspace as if its keys were all there are, with the maximum of its scores and the sum of its weights, and
+// attn_join_kernel adds the results up by their share of the whole sum.  How long a range is, is decided on the
 // device from the lengths (item_of), a multiple of `grain` and not below `chunk`, of which n_split cover the cache.
 struct RunsCall {
     KvView c;
     RunsView R;
     const int32_t* parent;
     const float *q, *qfull;
-    float *att, *acc, *ml; // acc [row][head][n_split][dh], ml [row][head][n_split][2] (log2 domain)
+    float *att, *acc, *ml; // acc [row][head][n_split][dh], ml [row][head][n_split][2] (maximum in the log2 domain, sum)
     uint32_t* chunk_used;  // one word of the workspace
     uint32_t hQ, G, n_split, chunk, grain, slots; // slots: items per KV head that fill the device
 };

@@ -27,7 +27,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(RunsCall a)
     const uint32_t n = __builtin_amdgcn_readfirstlane((min(u.pos + (row - u.r0) + 1, a.c.cap) + chunk - 1) / chunk);
     {
         const uint32_t h0 = blockIdx.y * 4 * HB + wave; // and every fourth behind it
-        float f[HB], inv[HB];
+        float f[HB], l[HB];
         size_t at[HB];
         vec gate[HB], o[HB];
 #pragma unroll
@@ -35,22 +35,22 @@ __global__ __launch_bounds__(256) void attn_join_kernel(RunsCall a)
             const size_t rh = (size_t)row * a.hQ + min(h0 + 4 * b, a.hQ - 1); // behind the last head that one again, not stored
             at[b] = rh * a.n_split;
             f[b] = AR_FLOOR;
-            inv[b] = 0.f;
+            l[b] = 0.f;
             if (lane < n) {
                 f[b] = a.ml[2 * (at[b] + lane)];
-                inv[b] = a.ml[2 * (at[b] + lane) + 1];
+                l[b] = a.ml[2 * (at[b] + lane) + 1];
             }
             if (a.qfull) gate[b] = *(const vec*)(a.qfull + rh * 2 * DH + DH + PER * lane);
 #pragma unroll
             for (uint32_t e = 0; e < PER; e++) o[b][e] = 0.f;
         }
-        // exp2 of a difference of maxima: NaN where a range saw one, which the sums below carry on
+        // a range's share of the whole sum; NaN where a range saw one, which the sums below carry on
 #pragma unroll
         for (uint32_t b = 0; b < HB; b++) {
             const float top = wave_max(f[b]);
-            f[b] = lane < n ? __builtin_amdgcn_exp2f(f[b] - top) : 0.f;
-            const float sum = wave_sum(inv[b] * f[b]);
-            inv[b] = sum == 0.f ? 0.f : 1.f / sum;
+            f[b] = lane < n ? __builtin_amdgcn_exp2f(f[b] - top) * l[b] : 0.f;
+            const float sum = wave_sum(f[b]);
+            f[b] *= sum == 0.f ? 0.f : 1.f / sum;
         }
         for (uint32_t s0 = 0; s0 < n; s0 += 4) {
             vec x[HB][4];
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(RunsCall a)
 #pragma unroll
         for (uint32_t b = 0; b < HB; b++) {
             if (h0 + 4 * b >= a.hQ) continue; // uniform
-            vec v = o[b] * inv[b];
+            vec v = o[b];
             if (a.qfull) {
 #pragma unroll
                 for (uint32_t e = 0; e < PER; e++) v[e] *= 1.f / (1.f + expf(-gate[b][e]));

@@ -13,12 +13,13 @@
 // One barrier per tile.  Matrix work per key and row: 4 dh operations times the products of split operands.
 //   F16 cache   K and V are operands as they are, Q and P are hi + lo halves: two products.
 //   F32 cache   every row of K and V is divided by the power of two that brings its largest value into [1, 2) and split
-//               into hi + lo halves, three products (lo . lo is below 2^-22 of its term).  The powers of two go back in where they
-//               cost nothing: a key's and a query's, added, into their scores (a product of both as factors would pass fp32's range
-//               where the score does not), a value row's into the exponent of its weight -- P V = (P 2^e)
-//               (V 2^-e), so the running maximum is kept over score + e -- and out of the sum again.  So fp32's range holds,
-//               row by row, with half the matrix work of three bf16 pieces.
-// Weights are kept around 2^6 rather than 1, which keeps the lo halves of small ones normal; the sum has the same factor.
+//               into hi + lo halves, three products (lo . lo is below 2^-22 of its term): half the matrix work of three bf16
+//               pieces.  The powers of two go back in where they cost little: a key's and a query's, added, into their scores (a
+//               product of both as factors would pass fp32's range where the score does not), a value row's into its weight,
+//               P V = (P 2^e) (V 2^-e).  The sum is of the weights P alone, against the maximum of the scores alone: with 2^e in
+//               it a row of small values beside large ones would fall out of it.  The weights that are multiplied have a power
+//               of two of their own per query row, 2^-vx, which follows the largest P 2^e.
+// Weights are kept around 2^6 rather than 1, which keeps the lo halves of small ones normal (half caches: the sum has the same factor).
 //   Bound by the matrix cores, fed from LDS.  Prompts of 8191 and 3001 rows, fp32, 16 heads on 2 of 256: 1.88 ms, 3 x 332 TFLOP/s
 // of products where a large matrix product reaches 1091; three chunks of 777 .. 2048 rows behind up to 6000, half, 32 heads on 8 of 128:
 // 0.58 ms, 2 x 426 TFLOP/s.  A tile of 32 fp32 keys takes 2.2 to 2.8 us, 64 half keys 3.4 us.  A call of a few tiles is a
@@ -33,12 +34,13 @@ typedef u32x2 __attribute__((may_alias)) lds_u32x2;
 typedef f32x4 __attribute__((may_alias)) lds_f32x4;
 typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 typedef i32x4 __attribute__((may_alias)) lds_i32x4;
+typedef int32_t __attribute__((may_alias)) lds_i32;
 
 constexpr uint32_t TL_M = AR_TILE_ROWS;
 // The running maximum is moved only when a score passes it by more than 2^TL_SLACK: weights stay below 2^(TL_UP + TL_SLACK), inside a
 // half's range, and most tiles need neither an exchange between lanes nor a rescaling of the accumulators.
-constexpr float TL_UP = 6.f, TL_SLACK = 8.f;
-constexpr int TL_VMIN = -90; // smallest exponent of a value row: a row of zeros keeps its weight in the sum
+constexpr float TL_UP = 6.f, TL_SLACK = 8.f, TL_TOP = 16384.f; // 2^(TL_UP + TL_SLACK)
+constexpr int TL_VX = 1000; // vx stays above -TL_VX
 
 template <int DH, bool F32>
 struct TileGeom {
@@ -50,7 +52,7 @@ struct TileGeom {
     static constexpr uint32_t KB = BN * DH * 2, VB = KB;           // bytes of one copy of K, of V^T
     static constexpr uint32_t RL = F32 ? 8 : 16, QL = 64 / RL;     // staging K: rows, and pieces of each, per wave and load
     static constexpr uint32_t PI = LPR / QL, KR = 8 / PI;          // loads per row, rows per thread
-    static constexpr uint32_t EXP = F32 ? 3 * BN * 4 : 0;          // per key: exponent of the score, exponent and factor of the value row
+    static constexpr uint32_t EXP = F32 ? 2 * BN * 4 : 0;          // per key: exponents of the score and of the value row
     static constexpr uint32_t BUF = NH * (KB + VB) + EXP + 64;     // + flags [4 NB]
     // Operand fragments read ahead of the products, and whether that order is pinned: left to itself the scheduler keeps two in flight,
     // which costs dh 256 4 % and suits halves with dh 128; fp32 with dh 128 has registers for one only.
@@ -147,9 +149,13 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
     const uint32_t wr = WR * wave; // the wave's first row in the block
     const bool has = wr < nr;      // uniform: a wave without rows only stages tiles
     // this lane's rows' positions behind node0 (below 128), 255 for a row that is not there: a byte for each block, so one register
-    uint32_t nodes = 0;
+    auto nodes_of = [&](uint32_t col) {
+        uint32_t n = 0;
 #pragma unroll
-    for (uint32_t rt = 0; rt < RT; rt++) nodes |= (wr + 16 * rt + m < nr ? (f0 + wr + 16 * rt + m) / a.G - node0 : 0xFFu) << (8 * rt);
+        for (uint32_t rt = 0; rt < RT; rt++) n |= (wr + 16 * rt + col < nr ? (f0 + wr + 16 * rt + col) / a.G - node0 : 0xFFu) << (8 * rt);
+        return n;
+    };
+    uint32_t nodes = nodes_of(m);
     const uint32_t first_node = (f0 + min(wr, nr - 1)) / a.G, last_node = (f0 + min(wr + WR, nr) - 1) / a.G;
 
     // Which of the four keys from `key` on this lane's row of block rt sees, pages aside.
@@ -157,7 +163,11 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
         const uint32_t node = nodes >> (8 * rt) & 0xFFu;
         const uint32_t stop = node == 0xFFu ? 0u : TREE ? k_end : min(k_end, u.pos + node0 + node + 1);
         uint32_t four = (1u << (stop > key ? min(stop - key, 4u) : 0u)) - 1u;
-        if (TREE) four &= k_end > u.pos ? tree_four(s_kin[min(node, TL_M - 1)], (int32_t)(key - u.pos)) : 15u;
+        if (TREE && k_end > u.pos) {
+            uint32_t at = node & (TL_M - 1);
+            asm("" : QK_REG(at), QK_REG(key)); // the row's address is not kept through the loop: registers
+            four &= tree_four(s_kin[at], (int32_t)(key - u.pos));
+        }
         return four;
     };
     bool odd_values = false; // uniform: some value of this range is not finite
@@ -208,6 +218,8 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
         uint8_t* s_v = buf + T::NH * T::KB;
         float* s_e = (float*)(buf + T::NH * (T::KB + T::VB));
         uint32_t* s_flag = (uint32_t*)(buf + T::NH * (T::KB + T::VB) + T::EXP);
+        uint32_t t = threadIdx.x, any = tile;
+        asm("" : QK_REG(t), QK_REG(any)); // places of exponents are computed per tile, not kept through the loop: registers
         if (!is_v) {
 #pragma unroll
             for (uint32_t j = 0; j < T::KR; j++) {
@@ -223,7 +235,7 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
                     mx = xor_lanes_max(mx);
                     const int ex = top_exponent(mx);
                     const float scale = pow2i(-ex);
-                    if (kq == 0) s_e[row] = u2f((uint32_t)ex);
+                    if (kq == 0) s_e[(wave % (T::WAVES / 2)) * T::RL * T::KR + t % T::RL + T::RL * j] = u2f((uint32_t)ex); // row
                     at += kq / 2 * 256 + kq % 2 * 8;
 #pragma unroll
                     for (uint32_t i = 0; i < T::PI; i++) { // pieces kq + 8 i: step i of 32 dims
@@ -270,13 +282,9 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
             float sc2[2];
 #pragma unroll
             for (uint32_t k = 0; k < 2; k++) {
-                const int e = max(top_exponent(u2f(top[k])), TL_VMIN);
+                const int e = top_exponent(u2f(top[k]));
                 sc2[k] = pow2i(-e);
-                if (piece < 4) { // row 4 k + piece of the eight
-                    float* at = s_e + 32 * st + 4 * sg + 16 * k + piece;
-                    at[BN] = (float)e;
-                    at[2 * BN] = sc2[k];
-                }
+                if (piece < 4) s_e[BN + 32 * st + 4 * (t / LPR % 4) + 16 * k + piece] = u2f((uint32_t)e); // row 4 k + piece of the eight
             }
             quad_spread(sc2, sc);
         } else if (!tile_whole(tile) || __builtin_amdgcn_ballot_w64(bad_pages != 0)) { // uniform
@@ -325,7 +333,10 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
     pages(0);
     // (and multiplied by log2 e / sqrt dh: scores are in the log2 domain)
     half8 qh[RT][KS], ql[RT][KS];
-    int q_exp[RT];
+    int xq[RT]; // exponents in one register: the query row's, and above it vx (fp32: o is held divided by 2^(vx - TL_UP))
+    auto q_exp = [&](uint32_t rt) { return (int)(int16_t)xq[rt]; };
+    auto v_exp = [&](uint32_t rt) { return xq[rt] >> 16; };
+    auto set_v_exp = [&](uint32_t rt, int v) { xq[rt] = (v << 16) | (xq[rt] & 0xFFFF); };
     const float qs = AR_LOG2E / sqrtf((float)DH);
     f32x4 qx[RT][KS][2];
 #pragma unroll
@@ -348,8 +359,8 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
         for (uint32_t ks = 0; ks < KS; ks++)
 #pragma unroll
             for (uint32_t j = 0; j < 8; j++) mx = fmaxf(mx, fabsf(qx[rt][ks][j / 4][j % 4]));
-        q_exp[rt] = top_exponent(xor_lanes_max(mx) * qs);
-        const float scale = pow2i(-q_exp[rt]);
+        xq[rt] = top_exponent(xor_lanes_max(mx) * qs);
+        const float scale = pow2i(-xq[rt]);
 #pragma unroll
         for (uint32_t ks = 0; ks < KS; ks++) {
             float y[8];
@@ -413,18 +424,12 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
 #pragma unroll
         for (uint32_t b = 0; b < 2; b++) {
             i32x4 ke;
-            f32x4 ve;
-            if constexpr (F32) {
-                const uint32_t j = 32 * sp + 16 * b + 4 * g;
-                ke = *(const lds_i32x4*)(s_e + j);
-                ve = *(const lds_f32x4*)(s_e + BN + j);
-            }
+            if constexpr (F32) ke = *(const lds_i32x4*)(s_e + 32 * sp + 16 * b + 4 * g);
 #pragma unroll
             for (uint32_t r = 0; r < 4; r++) {
 #pragma unroll
                 for (uint32_t rt = 0; rt < RT; rt++) {
-                    if constexpr (F32) s[rt][b][r] = __builtin_ldexpf(s[rt][b][r], ke[r] + q_exp[rt]) + ve[r];
-                    else s[rt][b][r] = __builtin_ldexpf(s[rt][b][r], q_exp[rt]);
+                    s[rt][b][r] = __builtin_ldexpf(s[rt][b][r], F32 ? ke[r] + q_exp(rt) : q_exp(rt));
                 }
             }
         }
@@ -454,9 +459,15 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
 #pragma unroll
             for (uint32_t rt = 0; rt < RT; rt++) {
                 const float top = xor_lanes_max(mx[rt]), m_new = top > m_run[rt] + TL_SLACK ? top : m_run[rt];
-                const float corr = __builtin_amdgcn_exp2f(m_run[rt] - m_new);
+                const float step = m_new - m_run[rt];
+                float corr = __builtin_amdgcn_exp2f(-step);
                 m_run[rt] = m_new;
                 l_run[rt] *= corr;
+                if constexpr (F32) { // the largest P 2^e need not have moved with the maximum
+                    const int was = v_exp(rt), vx = step < 1e30f ? max(was - (int)fminf(step, (float)TL_VX), -TL_VX) : was; // else: the first time
+                    set_v_exp(rt, vx);
+                    corr = __builtin_amdgcn_exp2f((float)(was - vx) - step);
+                }
 #pragma unroll
                 for (uint32_t n = 0; n < NT; n++) o[rt][n] *= corr;
             }
@@ -464,17 +475,47 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
         half8 ph[RT], pl[RT];
 #pragma unroll
         for (uint32_t rt = 0; rt < RT; rt++) {
-            const float top = m_run[rt] - TL_UP;
             float sum = 0.f, p[8];
+            if constexpr (F32) {
+                float big = 0.f;
+                const int up = (int)TL_UP - v_exp(rt);
 #pragma unroll
-            for (uint32_t b = 0; b < 2; b++) {
-                f32x4 vi;
-                if constexpr (F32) vi = *(const lds_f32x4*)(s_e + 2 * BN + 32 * sp + 16 * b + 4 * g);
+                for (uint32_t b = 0; b < 2; b++) {
+                    const i32x4 ve = *(const lds_i32x4*)(s_e + BN + 32 * sp + 16 * b + 4 * g);
 #pragma unroll
-                for (uint32_t r = 0; r < 4; r++) {
-                    p[4 * b + r] = __builtin_amdgcn_exp2f(s[rt][b][r] - top);
-                    if constexpr (F32) sum += p[4 * b + r] * vi[r];
-                    else sum += p[4 * b + r];
+                    for (uint32_t r = 0; r < 4; r++) {
+                        const float x = __builtin_amdgcn_exp2f(s[rt][b][r] - m_run[rt]);
+                        sum += x;
+                        p[4 * b + r] = __builtin_ldexpf(x, ve[r] + up);
+                        big = fmaxf(big, p[4 * b + r]);
+                    }
+                }
+                if (__builtin_amdgcn_ballot_w64(big > 1.01f * TL_TOP)) { // uniform: now and then
+                    float top = -(float)TL_VX; // the largest P 2^e, as an exponent
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; i++) {
+                        const int e = ((const lds_i32*)s_e)[BN + 32 * sp + 16 * (i / 4) + 4 * g + i % 4];
+                        top = fmaxf(top, s[rt][i / 4][i % 4] - m_run[rt] + (float)e);
+                    }
+                    top = fminf(xor_lanes_max(top), (float)TL_VX);
+                    const int was = v_exp(rt), vx = top > (float)was + TL_SLACK ? (int)__builtin_ceilf(top) : was;
+                    set_v_exp(rt, vx);
+#pragma unroll
+                    for (uint32_t n = 0; n < NT; n++)
+#pragma unroll
+                        for (uint32_t r = 0; r < 4; r++) o[rt][n][r] = __builtin_ldexpf(o[rt][n][r], was - vx);
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; i++) {
+                        const int e = ((const lds_i32*)s_e)[BN + 32 * sp + 16 * (i / 4) + 4 * g + i % 4];
+                        p[i] = __builtin_ldexpf(__builtin_amdgcn_exp2f(s[rt][i / 4][i % 4] - m_run[rt]), e + (int)TL_UP - vx);
+                    }
+                }
+            } else {
+                const float top = m_run[rt] - TL_UP;
+#pragma unroll
+                for (uint32_t i = 0; i < 8; i++) {
+                    p[i] = __builtin_amdgcn_exp2f(s[rt][i / 4][i % 4] - top);
+                    sum += p[i];
                 }
             }
             l_run[rt] += sum; // of this lane's keys; the lane groups are added at the end
@@ -503,6 +544,12 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
     if (n_tile > 1) fetch(1);
     if (n_tile > 2) pages(2);
     __syncthreads();
+    if constexpr (F32) { // vx begins at the smallest exponent of the first tile's value rows: no row's weights are made small for the sake of one it does not see
+        const float* s_e = (const float*)(s_dyn + T::NH * (T::KB + T::VB));
+        const int least = -(int)wave_max(-(float)((const lds_i32*)s_e)[BN + lane % BN]);
+#pragma unroll
+        for (uint32_t rt = 0; rt < RT; rt++) set_v_exp(rt, least);
+    }
     for (uint32_t tile = 0; tile < n_tile; tile++) {
         const uint8_t* buf = s_dyn + (tile & 1u) * T::BUF;
         const uint32_t* s_flag = (const uint32_t*)(buf + T::NH * (T::KB + T::VB) + T::EXP);
@@ -524,6 +571,9 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
         __syncthreads();
     }
     if (!has) return; // the whole wave; no barrier below
+    uint32_t me = threadIdx.x & 15u;
+    asm("" : QK_REG(me)); // the rows' places are computed anew from here on, not kept through the loop: registers
+    nodes = nodes_of(me);
     if (odd_values) { // rare: values that are not finite were taken out of the products; they reach the rows that see them here
         for (uint32_t key0 = k_begin; key0 < k_end; key0 += 4) { // from a multiple of four: one page
             const uint32_t page = kv_page(a.c, u.seq, key0);
@@ -548,10 +598,10 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
 #pragma unroll
     for (uint32_t rt = 0; rt < RT; rt++) {
         const float l = xor_lanes_sum(l_run[rt]);
-        const uint32_t f = wr + 16 * rt + m;
+        const uint32_t f = wr + 16 * rt + me;
         if (f >= nr) continue;
         const size_t rh = (size_t)(u.r0 + (f0 + f) / a.G) * a.hQ + kv * a.G + (f0 + f) % a.G;
-        const float inv = a.n_split > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
         float* out = a.n_split > 1 ? a.acc + (rh * a.n_split + split) * DH : a.att + rh * DH;
         if (a.n_split > 1 && g == 0) {
             a.ml[2 * (rh * a.n_split + split)] = m_run[rt];
@@ -566,7 +616,10 @@ __global__ __launch_bounds__((64 * TileGeom<DH, F32>::WAVES), 2) void attn_tile_
                     const uint32_t d = E * (16 * c + 4 * g + r) + e;
                     f32x4 x;
 #pragma unroll
-                    for (uint32_t i = 0; i < 4; i++) x[i] = o[rt][(e + i) * NC + c][r] * inv;
+                    for (uint32_t i = 0; i < 4; i++) {
+                        x[i] = o[rt][(e + i) * NC + c][r] * inv;
+                        if constexpr (F32) x[i] = __builtin_ldexpf(x[i], v_exp(rt) - (int)TL_UP);
+                    }
                     if (a.n_split == 1 && a.qfull) {
                         const f32x4 gt = *(const f32x4*)(a.qfull + rh * 2 * DH + DH + d);
 #pragma unroll

@@ -530,3 +530,32 @@ def _sizes_cancel(p):
 RANGE_SCORE = [(f"{what}, {where}", case, edit) for what, edit in [("keys and queries of size 2^70 in dims of their own", _far_and_apart(70)),
                                                                   ("keys 2^100, queries 2^-100", _sizes_cancel(100)), ("keys 2^-100, queries 2^100", _sizes_cancel(-100))]
                for where, case in FORMS]
+
+
+def _rows_of_size(every, small, large):
+    """Cache rows 0, every, 2 every ... have values of size `small`, the others of size `large` (as powers of two; None: zeros)."""
+    def edit(x):
+        for s in range(len(x["seq"])):
+            for r in range(x["c"]["len"][s]):
+                p = small if r % every == 0 else large
+                page, at = place(x["c"], s, r)
+                x["c"]["v"][:, page, :, at] *= np.float32(0 if p is None else 2.0 ** p)
+    return edit
+
+
+def _first_rows_zero(n, p):
+    """The first n rows of a sequence are zeros, the others of size 2^p: a whole tile, or a whole range of keys, of either."""
+    def edit(x):
+        for s in range(len(x["seq"])):
+            for r in range(x["c"]["len"][s]):
+                page, at = place(x["c"], s, r)
+                x["c"]["v"][:, page, :, at] *= np.float32(2.0 ** p if r >= n else 0)
+    return edit
+
+
+RANGE_SUM = [(f"{what}, {where}", case, edit)
+             for what, edit in [("every other row zero beside 2^60", _rows_of_size(2, None, 60)), ("every other row zero beside 2^110", _rows_of_size(2, None, 110)),
+                                ("every third row 2^-100 beside 2^100", _rows_of_size(3, -100, 100)), ("one row in seven 2^100 beside 2^-100", _rows_of_size(7, 100, -100)),
+                                ("the first 32 rows zero, then 2^50", _first_rows_zero(32, 50)), ("the first 64 rows zero, then 2^44", _first_rows_zero(64, 44)),
+                                ("the first 64 rows zero, then 2^110", _first_rows_zero(64, 110))]
+             for where, case in FORMS if "64" not in what or "one range" not in where]

@@ -284,3 +284,8 @@ def test_side_stream(qk, dev, up, ws):
 @pytest.mark.parametrize("name,case,edit", KC.RANGE_SCORE, ids=[c[0] for c in KC.RANGE_SCORE])
 def test_scores_of_far_keys_and_queries(qk, up, ws, name, case, edit):
     KC.range_case(qk, up, ws, case, edit, "row")
+
+
+@pytest.mark.parametrize("name,case,edit", KC.RANGE_SUM, ids=[c[0] for c in KC.RANGE_SUM])
+def test_value_rows_of_any_size_keep_their_weight(qk, up, ws, name, case, edit):
+    KC.range_case(qk, up, ws, case, edit, "row")

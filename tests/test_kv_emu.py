@@ -63,3 +63,8 @@ def test_results_do_not_depend_on_the_order_of_the_threads(qk, emu):
 @pytest.mark.parametrize("name,case,edit", KC.RANGE_SCORE, ids=[c[0] for c in KC.RANGE_SCORE])
 def test_scores_of_far_keys_and_queries(qk, emu, name, case, edit):
     KC.range_case(qk, emu.tensor, emu.workspace, case, edit, "row")
+
+
+@pytest.mark.parametrize("name,case,edit", KC.RANGE_SUM, ids=[c[0] for c in KC.RANGE_SUM])
+def test_value_rows_of_any_size_keep_their_weight(qk, emu, name, case, edit):
+    KC.range_case(qk, emu.tensor, emu.workspace, case, edit, "row")
