@@ -14,8 +14,8 @@
 // The query rows of a run that share a KV head (positions x heads of the group) are numbered f = position * G + head, so
 // any group size fills the 16 columns.
 //
-// Two halves hold an fp32 value to 2^-22 inside a half's range, three bf16 pieces hold it exactly in fp32's own range:
-// products of split operands give fp32 results on the matrix cores (the kernels say which they use and why).
+// Two halves hold an fp32 value to 2^-22 where the lo half is normal (from 2^-2 up; below it to 2^-25 absolute), three bf16 pieces
+// hold it exactly in fp32's own range: products of split operands on the matrix cores (the kernels say which they use and why).
 #pragma once
 #include "qk_kv.h"
 #include "qk_mfma.h"
@@ -180,7 +180,7 @@ __device__ __forceinline__ Bf3 split3(const float* x)
     return r;
 }
 
-// Eight floats as hi + lo halves, both rounded to nearest: exact to 2^-22 of x while x is inside a half's normal range.  Two values
+// Eight floats as hi + lo halves, both rounded to nearest: exact to 2^-22 of x from |x| = 2^-2 up to a half's largest, below to 2^-25.  Two values
 // take three instructions: one packs both hi halves, and the rest x * s - hi is formed and rounded by one mixed-precision
 // multiply-add each.  The pinned register keeps the compiler from converting every value a second time on its own, the pinned
 // factor 1 from turning the multiply-add into a subtraction of converted values.
@@ -216,10 +216,11 @@ __device__ __forceinline__ Half2 split2(const float* x)
     return Half2{__builtin_bit_cast(half8, h), __builtin_bit_cast(half8, l)};
 }
 
-// The power of two that brings a maximum of magnitudes into [1, 2): its exponent, limited to what the reciprocal can hold.
+// Exponent of the power of two that a row is divided by, so that its largest magnitude m comes into [2^14, 2^15): as high as a
+// half allows, since elements below 2^-2 lose bits.  Not below -126, so that the power and its reciprocal are normal.
 __device__ __forceinline__ int top_exponent(float m)
 {
-    return min(max((int)(f2u(m) >> 23) - 127, -126), 126);
+    return max((int)(f2u(m) >> 23) - 127 - 14, -126);
 }
 __device__ __forceinline__ float pow2i(int e) { return u2f((uint32_t)(e + 127) << 23); }
 

@@ -12,14 +12,16 @@
 //        that the weights P have in the registers of the first product, 16 bytes per dim.
 // One barrier per tile.  Matrix work per key and row: 4 dh operations times the products of split operands.
 //   F16 cache   K and V are operands as they are, Q and P are hi + lo halves: two products.
-//   F32 cache   every row of K and V is divided by the power of two that brings its largest value into [1, 2) and split
-//               into hi + lo halves, three products (lo . lo is below 2^-22 of its term): half the matrix work of three bf16
-//               pieces.  The powers of two go back in where they cost little: a key's and a query's, added, into their scores (a
+//   F32 cache   every row of K and V is divided by the power of two that brings its largest value into [2^14, 2^15) and
+//               split into hi + lo halves, three products (lo . lo is below 2^-22 of its term): half the matrix work of three
+//               bf16 pieces.  The powers of two go back in where they cost little: a key's and a query's, added, into their scores (a
 //               product of both as factors would pass fp32's range where the score does not), a value row's into its weight,
 //               P V = (P 2^e) (V 2^-e).  The sum is of the weights P alone, against the maximum of the scores alone: with 2^e in
 //               it a row of small values beside large ones would fall out of it.  The weights that are multiplied have a power
 //               of two of their own per query row, 2^-vx, which follows the largest P 2^e.
-// Weights are kept around 2^6 rather than 1, which keeps the lo halves of small ones normal (half caches: the sum has the same factor).
+// What two halves hold is to 2^-22 exact while the lo half is normal, so everything that is split lies as high in a half's range as it may
+// (sums are fp32: 2^15 2^15 times the keys): elements down to 2^-16 of their row's largest are exact to 2^-22, smaller ones to 2^-39
+// of that; weights around 2^11, not 1, are to 2^-36 of the row's largest (half caches: the sum has the same factor).
 //   Bound by the matrix cores, fed from LDS.  Prompts of 8191 and 3001 rows, fp32, 16 heads on 2 of 256: 1.88 ms, 3 x 332 TFLOP/s
 // of products where a large matrix product reaches 1091; three chunks of 777 .. 2048 rows behind up to 6000, half, 32 heads on 8 of 128:
 // 0.58 ms, 2 x 426 TFLOP/s.  A tile of 32 fp32 keys takes 2.2 to 2.8 us, 64 half keys 3.4 us.  A call of a few tiles is a
@@ -38,8 +40,9 @@ typedef int32_t __attribute__((may_alias)) lds_i32;
 
 constexpr uint32_t TL_M = AR_TILE_ROWS;
 // The running maximum is moved only when a score passes it by more than 2^TL_SLACK: weights stay below 2^(TL_UP + TL_SLACK), inside a
-// half's range, and most tiles need neither an exchange between lanes nor a rescaling of the accumulators.
-constexpr float TL_UP = 6.f, TL_SLACK = 8.f, TL_TOP = 16384.f; // 2^(TL_UP + TL_SLACK)
+// half's range, and most tiles need neither an exchange between lanes nor a rescaling of the accumulators.  What is left above the maximum is
+// lost below it: with 2^13 and 2^2 prompts of 8191 and 3001 rows take 1.05 of the time with 2^6 and 2^8, so 1.03.
+constexpr float TL_UP = 11.f, TL_SLACK = 4.f, TL_TOP = 32768.f; // 2^(TL_UP + TL_SLACK)
 constexpr int TL_VX = 1000; // vx stays above -TL_VX
 
 template <int DH, bool F32>

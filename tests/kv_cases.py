@@ -559,3 +559,65 @@ RANGE_SUM = [(f"{what}, {where}", case, edit)
                                 ("the first 32 rows zero, then 2^50", _first_rows_zero(32, 50)), ("the first 64 rows zero, then 2^44", _first_rows_zero(64, 44)),
                                 ("the first 64 rows zero, then 2^110", _first_rows_zero(64, 110))]
              for where, case in FORMS if "64" not in what or "one range" not in where]
+
+
+FORMS16 = [("halves, many rows", ("f16", 128, 8, 2, 16, 160, (20, 9), (90, 65), False, 0)), ("halves, many rows, one range", ("f16", 256, 8, 1, 0, 64, (20, 9), (43, 40), True, 0)),
+           ("halves, wide tree", ("f16", 256, 8, 2, 16, 192, (20, 9), (120, 65), False, 2)), ("halves, few rows", ("f16", 128, 4, 2, 16, 160, (5, 1), (140, 65), False, 2))]
+
+
+def _value_dim(p):
+    """One dim of all value rows is 2^p times as large as the others."""
+    def edit(x):
+        x["c"]["v"][..., 0] *= np.float32(2.0 ** p)
+    return edit
+
+
+def _value_dim_of_a_row(p):
+    """One dim of one value row is 2^p times as large as everything else."""
+    def edit(x):
+        for s in range(len(x["seq"])):
+            page, at = place(x["c"], s, 2)
+            x["c"]["v"][:, page, :, at, 5] *= np.float32(2.0 ** p)
+    return edit
+
+
+def _key_dim(p):
+    """One dim of the keys is 2^p times as large as the others, that of the queries as much smaller."""
+    def edit(x):
+        x["c"]["k"][..., 0] *= np.float32(2.0 ** p)
+        x["q"][..., 0] *= np.float32(2.0 ** -p)
+    return edit
+
+
+def _query_dim(p):
+    """One dim of the queries is 2^p times as large as the others, that of the keys as much smaller."""
+    def edit(x):
+        x["q"][..., 0] *= np.float32(2.0 ** p)
+        x["c"]["k"][..., 0] *= x["c"]["k"].dtype.type(2.0 ** -p)
+    return edit
+
+
+def _sink(bits):
+    """The first key takes nearly the whole weight, 2^bits times that of any other, and its values are zeros."""
+    def edit(x):
+        c, dh = x["c"], x["q"].shape[2]
+        x["q"] *= np.float32(0.05)
+        x["q"][..., 1] = 8
+        c["k"][..., 1] = 0
+        for s in range(len(x["seq"])):
+            page, at = place(c, s, 0)
+            c["k"][:, page, :, at] = 0
+            c["k"][:, page, :, at, 1] = bits * np.log(2) * np.sqrt(dh) / 8
+            c["v"][:, page, :, at] = 0
+    return edit
+
+
+# Operands held as two halves are exact to 2^-22 down to 2^-16 of their row's largest and to 2^-39 of that below; a product's weights
+# likewise, to 2^-36 of the row's largest.  At 2^-20 (values) and 2^-17 (weights) of the largest that is 2^-19 of the element, half of
+# the 4e-6 of the whole result.
+RANGE_SPLIT = [(f"{what}, {where}", case, edit, per) for what, edit, per in
+               [("a value dim 2^6", _value_dim(6), "dim"), ("a value dim 2^14", _value_dim(14), "dim"), ("a value dim 2^20", _value_dim(20), "dim"),
+                ("a value 2^14", _value_dim_of_a_row(14), "dim"), ("a value 2^17", _value_dim_of_a_row(17), "dim"),
+                ("a key dim 2^10", _key_dim(10), "row"), ("a key dim 2^16", _key_dim(16), "row")] for where, case in FORMS]
+RANGE_SPLIT += [(f"{what}, {where}", case, edit, "row") for what, edit in [("a query dim 2^10", _query_dim(10)), ("a query dim 2^14", _query_dim(14)),
+                                                                           ("a key with the weight, 2^17", _sink(17))] for where, case in FORMS + FORMS16]

@@ -68,3 +68,8 @@ def test_scores_of_far_keys_and_queries(qk, emu, name, case, edit):
 @pytest.mark.parametrize("name,case,edit", KC.RANGE_SUM, ids=[c[0] for c in KC.RANGE_SUM])
 def test_value_rows_of_any_size_keep_their_weight(qk, emu, name, case, edit):
     KC.range_case(qk, emu.tensor, emu.workspace, case, edit, "row")
+
+
+@pytest.mark.parametrize("name,case,edit,per", KC.RANGE_SPLIT, ids=[c[0] for c in KC.RANGE_SPLIT])
+def test_small_elements_beside_large_ones(qk, emu, name, case, edit, per):
+    KC.range_case(qk, emu.tensor, emu.workspace, case, edit, per)
