@@ -480,8 +480,8 @@ int qkk_attn_prep_axes(const qkk_kv_cache *C_host, uint32_t layer, const qkk_kv_
  * 2^-13 of the row's largest, and to 2^-36 of that below.  Otherwise an F32 cache's operands are exact.
  * The same call gives the same bits.  Into how many ranges the keys are cut, and with it the last bits of a
  * row, depends on the lengths of all runs of the call.
- *   workspace: qkk_attn_runs_workspace_bytes(), 256-byte aligned, no initialisation needed; calls (and
- *   graphs) that share one must not overlap in time. */
+ *   workspace: qkk_attn_runs_workspace_bytes() (0 for sizes that the calls refuse), 256-byte aligned, no
+ *   initialisation needed; calls (and graphs) that share one must not overlap in time. */
 #define QKK_TREE_MAX 256u
 size_t qkk_attn_runs_workspace_bytes(const qkk_kv_cache *C_host, const qkk_kv_runs *R_host, uint32_t hQ);
 int qkk_attn_packed(const qkk_kv_cache *C_host, uint32_t layer, const qkk_kv_runs *R_host, const float *qhat,

@@ -170,6 +170,8 @@ extern "C" {
 size_t qkk_attn_runs_workspace_bytes(const qkk_kv_cache* C, const qkk_kv_runs* R, uint32_t hQ)
 {
     if (!C || !R || !C->n_kv || hQ < C->n_kv || !C->seq_pages || !C->page_rows) return 0;
+    // what the calls refuse: the sums below are not made for it
+    if ((uint64_t)C->seq_pages * C->page_rows > (1u << 30) || R->n_rows > (1u << 20) || R->n_run > (1u << 20) || hQ > 4096 || C->dh > 256) return 0;
     const Plan p = plan_of(C, R, hQ);
     return (p.n_split > 1 ? (size_t)R->n_rows * hQ * p.n_split * (C->dh + 2) * sizeof(float) : 0) + 256;
 }

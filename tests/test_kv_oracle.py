@@ -230,3 +230,19 @@ def test_bounds_of_the_checks_hold_for_the_oracle():
     wrong = OK.attend(OK.Cache(c.k * np.float32(1.001), c.v, None), 0, rows, q)
     with pytest.raises(AssertionError):
         KC.check_att(wrong.astype(np.float32), want, tol, rows)
+
+
+@pytest.mark.parametrize("change", [dict(seq_pages=1 << 31, page_rows=1 << 16), dict(seq_pages=0xFFFFFFFF, page_rows=0xFFFFFFFF), dict(seq_pages=1 << 20, page_rows=1 << 16),
+                                    dict(dh=1 << 20)])
+def test_workspace_of_a_cache_that_the_calls_refuse(qk, change):
+    """Sizes whose ranges of keys do not fit 32 bits ended the process in a division by zero; 0 bytes are asked for."""
+    c, r = cache_struct(qk, **change), runs_struct(qk)
+    assert qk.lib().qkk_attn_runs_workspace_bytes(C.byref(c), C.byref(r), 4) == 0
+    assert qk.lib().qkk_attn_packed(C.byref(c), 0, C.byref(r), 16, None, 16, 256, 1 << 40, 4, None) == -2
+
+
+@pytest.mark.parametrize("change,hq", [(dict(n_rows=(1 << 20) + 1), 4), (dict(n_run=(1 << 20) + 1), 4), (dict(n_rows=0xFFFFFFFF, max_run=0xFFFFFFFF), 4), (dict(), 8192)])
+def test_workspace_of_runs_that_the_calls_refuse(qk, change, hq):
+    c, r = cache_struct(qk), runs_struct(qk, **change)
+    assert qk.lib().qkk_attn_runs_workspace_bytes(C.byref(c), C.byref(r), hq) == 0
+    assert qk.lib().qkk_attn_packed(C.byref(c), 0, C.byref(r), 16, None, 16, 256, 1 << 40, hq, None) == -2
