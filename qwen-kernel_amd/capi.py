@@ -108,7 +108,8 @@ def _signatures():
 
 def bind(L, partial=False):
     """Declares the C signatures on a loaded library.  partial: skip entry points the library does not
-    export (the tests' host-side build of some kernels)."""
+    export (the tests' host-side build of some kernels, whose tensors lie in host memory)."""
+    L.host_side = partial
     for name, (restype, argtypes) in _signatures().items():
         if partial and not hasattr(L, name):
             continue
@@ -578,6 +579,16 @@ def _here(who, dev):
             raise ValueError(f"{who}: the cache is on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
 
 
+def _stream_at(who, dev):
+    """The current stream for tensors on device number `dev`, which must not be host memory (-1) where there is a device to follow the
+    addresses.  Without a device the library says so itself."""
+    if dev < 0 and not lib().host_side:
+        import torch
+        if torch.cuda.is_available():
+            raise ValueError(f"{who}: the tensors are in host memory")
+    return _stream()
+
+
 def _bytes(who, t, dev):
     """(address, bytes) of a workspace."""
     return _want(who, "workspace", t, t.dtype, None, dev), t.numel() * t.element_size()
@@ -665,7 +676,7 @@ def attn_prep_axes(cache, layer, runs, q, kin, vin, q_norm_w, k_norm_w, rope, pa
         _want(who, "vin", vin, f, kv, dev), _want(who, "q_norm_w", q_norm_w, f, w, dev), _want(who, "k_norm_w", k_norm_w, f, w, dev),
         _want(who, "rope", rope, f, None, dev), rope_rows, _want(who, "pair_axis", pair_axis, cache.u8, (half,), dev), n_axis,
         _want(who, "axis_pos", axis_pos, cache.i32, (n_axis, rows), dev), _want(who, "qhat", qhat, f, (rows, hQ, dh), dev), hQ, 2 * half,
-        int(pitch != dh), eps, _stream()))
+        int(pitch != dh), eps, _stream_at(who, dev)))
     return qhat
 
 
@@ -687,10 +698,10 @@ def _attn_runs(who, cache, layer, runs, parent, qhat, workspace, qfull, att):
     gate = 0 if qfull is None else _want(who, "qfull", qfull, f, (rows, hQ, 2 * dh), dev)
     space, nbytes = _bytes(who, workspace, dev)
     if parent is None:
-        _check(lib().qkk_attn_packed(cache.ref_c, layer, runs.ref_c, q, gate, out, space, nbytes, hQ, _stream()))
+        _check(lib().qkk_attn_packed(cache.ref_c, layer, runs.ref_c, q, gate, out, space, nbytes, hQ, _stream_at(who, dev)))
     else:
         up = _want(who, "parent", parent, cache.i32, (rows,), dev)
-        _check(lib().qkk_attn_tree(cache.ref_c, layer, runs.ref_c, up, q, gate, out, space, nbytes, hQ, _stream()))
+        _check(lib().qkk_attn_tree(cache.ref_c, layer, runs.ref_c, up, q, gate, out, space, nbytes, hQ, _stream_at(who, dev)))
     return att
 
 
@@ -721,7 +732,7 @@ def kv_resize(cache, len_new, workspace, status=None):
         status = len_new.new_empty((1,))
     space, nbytes = _bytes(who, workspace, dev)
     _check(lib().qkk_kv_resize(cache.ref_c, _want(who, "len_new", len_new, cache.i32, (cache.n_seq,), dev),
-                               _want(who, "status", status, cache.i32, (1,), dev), space, nbytes, _stream()))
+                               _want(who, "status", status, cache.i32, (1,), dev), space, nbytes, _stream_at(who, dev)))
     return status
 
 
@@ -734,7 +745,7 @@ def kv_fork(cache, src, dst, workspace, status=None):
         status = src.new_empty((1,))
     space, nbytes = _bytes(who, workspace, dev)
     _check(lib().qkk_kv_fork(cache.ref_c, _want(who, "src", src, cache.i32, (n,), dev), _want(who, "dst", dst, cache.i32, (n,), dev), n,
-                             _want(who, "status", status, cache.i32, (1,), dev), space, nbytes, _stream()))
+                             _want(who, "status", status, cache.i32, (1,), dev), space, nbytes, _stream_at(who, dev)))
     return status
 
 
@@ -747,4 +758,4 @@ def kv_compact(cache, seq, base, path, n_path):
     _here(who, dev)
     wide = path.shape[1]
     _check(lib().qkk_kv_compact(cache.ref_c, _want(who, "seq", seq, i32, (n,), dev), _want(who, "base", base, i32, (n,), dev),
-                                _want(who, "path", path, i32, (n, wide), dev), _want(who, "n_path", n_path, i32, (n,), dev), n, wide, _stream()))
+                                _want(who, "path", path, i32, (n, wide), dev), _want(who, "n_path", n_path, i32, (n,), dev), n, wide, _stream_at(who, dev)))

@@ -246,3 +246,24 @@ def test_workspace_of_runs_that_the_calls_refuse(qk, change, hq):
     c, r = cache_struct(qk), runs_struct(qk, **change)
     assert qk.lib().qkk_attn_runs_workspace_bytes(C.byref(c), C.byref(r), hq) == 0
     assert qk.lib().qkk_attn_packed(C.byref(c), 0, C.byref(r), 16, None, 16, 256, 1 << 40, hq, None) == -2
+
+
+def test_host_tensors_do_not_reach_a_device(monkeypatch):
+    """A cache in host memory is consistent in itself, but its addresses are none of a device's: refused in front of the launch.  (Without a
+    device the library itself refuses; here torch is made to say that there is one.)"""
+    import torch
+
+    import __graft_entry__ as entry
+    qk = entry.load_package()
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(qk.capi, "_stream", lambda: None)
+    k, i32 = torch.zeros(1, 4, 2, 16, 128), lambda *v: torch.tensor(v, dtype=torch.int32)
+    cache, runs = qk.KvCache(k, k.clone(), len=i32(0, 0, 0, 0)), qk.KvRuns(3, i32(0, 3), i32(0), i32(0))
+    raw = torch.zeros(1 << 16, dtype=torch.uint8)
+    ws, q, kv, w = raw[-raw.data_ptr() % 256:], torch.zeros(3, 4, 128), torch.zeros(3, 2, 128), torch.zeros(128)
+    calls = [lambda: qk.attn_packed(cache, 0, runs, q, ws), lambda: qk.attn_tree(cache, 0, runs, i32(-1, 0, 0), q, ws), lambda: qk.kv_resize(cache, i32(1, 1, 1, 1), ws),
+             lambda: qk.kv_fork(cache, i32(0), i32(1), ws), lambda: qk.kv_compact(cache, i32(0), i32(0), i32(0, 1).view(1, 2), i32(2)),
+             lambda: qk.attn_prep_axes(cache, 0, runs, q, kv, kv, w, w, torch.zeros(8, 4, 2), torch.zeros(4, dtype=torch.uint8), i32(0, 1, 2).view(1, 3))]
+    for call in calls:
+        with pytest.raises(ValueError, match="host memory"):
+            call()
