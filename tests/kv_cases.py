@@ -621,3 +621,21 @@ RANGE_SPLIT = [(f"{what}, {where}", case, edit, per) for what, edit, per in
                 ("a key dim 2^10", _key_dim(10), "row"), ("a key dim 2^16", _key_dim(16), "row")] for where, case in FORMS]
 RANGE_SPLIT += [(f"{what}, {where}", case, edit, "row") for what, edit in [("a query dim 2^10", _query_dim(10)), ("a query dim 2^14", _query_dim(14)),
                                                                            ("a key with the weight, 2^17", _sink(17))] for where, case in FORMS + FORMS16]
+
+
+# ---- more runs than a wave looks over at once ------------------------------------------------------------------------------
+
+def many_runs(n_run, seed, longest, cap):
+    """Lengths and pasts of n_run runs, a third of them empty, the last ones too."""
+    rng = np.random.default_rng(seed)
+    lens = [int(n) if rng.random() > 0.33 else 0 for n in rng.integers(1, longest + 1, n_run)]
+    lens[-2:] = [0, 0]
+    lens[n_run // 2], lens[64 if n_run > 66 else 0] = longest, longest
+    return tuple(lens), tuple(int(p) for p in rng.integers(0, cap - longest, n_run))
+
+
+MANY_RUNS = [("f16", 128, 2, 1, 16, 160, *many_runs(65, 1, 4, 160), False, 1), ("f32", 128, 2, 1, 16, 160, *many_runs(130, 2, 3, 160), True, 2),
+             ("f16", 128, 4, 1, 16, 160, *many_runs(140, 3, 11, 160), False, 0), ("f32", 128, 4, 1, 0, 160, *many_runs(100, 4, 10, 160), False, 2),
+             ("f32", 128, 12, 1, 0, 48, *many_runs(70, 5, 12, 48), True, 0)]
+MANY_RUNS_PREP = [("f16", 128, 2, 1, 16, 64, (11, 11, 10), True, False, many_runs(140, 6, 3, 64)[0], many_runs(140, 6, 3, 60)[1], 2),
+                  ("f32", 256, 2, 1, 0, 64, (32,), False, True, many_runs(67, 7, 4, 64)[0], many_runs(67, 7, 4, 60)[1], 0)]

@@ -294,3 +294,13 @@ def test_value_rows_of_any_size_keep_their_weight(qk, up, ws, name, case, edit):
 @pytest.mark.parametrize("name,case,edit,per", KC.RANGE_SPLIT, ids=[c[0] for c in KC.RANGE_SPLIT])
 def test_small_elements_beside_large_ones(qk, up, ws, name, case, edit, per):
     KC.range_case(qk, up, ws, case, edit, per)
+
+
+@pytest.mark.parametrize("case", KC.MANY_RUNS, ids=lambda c: f"{c[0]}-{len(c[6])}-b{c[9]}")
+def test_attention_of_many_runs(qk, up, ws, case):
+    KC.att_case(qk, up, ws, case, behind=1)
+
+
+@pytest.mark.parametrize("case", KC.MANY_RUNS_PREP, ids=lambda c: f"{c[0]}-{len(c[9])}")
+def test_prep_of_many_runs(qk, up, case):
+    KC.prep_case(qk, up, case)
