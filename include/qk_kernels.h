@@ -470,8 +470,8 @@ int qkk_attn_prep_axes(const qkk_kv_cache *C_host, uint32_t layer, const qkk_kv_
  *                  run (below t); anything else makes the node a root.  max_run <= QKK_TREE_MAX.  A tree
  *                  of one node is the decode step.
  * A row that sees nothing gives zeros.  What a row does not see never enters its result, whatever the
- * cache holds there; what it sees and is not finite makes it NaN or infinite (a score of minus infinity is a
- * weight of zero).  Value rows of an F32 cache may differ in size as far as fp32 reaches (below 2^-126 they
+ * cache holds there; what it sees and is not finite makes it NaN or infinite (an infinite key, too; only a
+ * score of finite operands that passes fp32's range downwards is a weight of zero).  Value rows of an F32 cache may differ in size as far as fp32 reaches (below 2^-126 they
  * may count as zeros).
  * The softmax's maximum and sum and all sums are fp32.  Into the products go as two halves per element: the
  * queries, for an F16 cache the weights, and for an F32 cache, where a run may have more than 16 (dh 128: 32)
@@ -508,8 +508,9 @@ int qkk_attn_tree(const qkk_kv_cache *C_host, uint32_t layer, const qkk_kv_runs 
  * qkk_kv_compact for i < n: of the drafted rows behind cache row base[i] of sequence seq[i], row
  *                base + path[i][j] is moved to base + j, j < n_path[i] (path [n][max_path], ascending):
  *                the accepted path of a tree to the front.  A path that is not strictly ascending, or
- *                leaves the sequence's pages, is left out (nothing of it is moved).  Touches no books.  A
- *                sequence comes once per call (two paths of one race for its rows).  max_path <= QKK_TREE_MAX. */
+ *                leaves the sequence's pages, is left out (nothing of it is moved).  Touches no books: rows that
+ *                another sequence shares (a fork since they were added) change for it, too.  A sequence comes
+ *                once per call (two paths of one race for its rows).  max_path <= QKK_TREE_MAX. */
 size_t qkk_kv_workspace_bytes(const qkk_kv_cache *C_host);
 int qkk_kv_resize(const qkk_kv_cache *C_host, const int32_t *len_new, int32_t *status, void *workspace,
                   size_t workspace_bytes, void *stream);

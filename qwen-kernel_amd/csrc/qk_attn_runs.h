@@ -60,8 +60,8 @@ __device__ __forceinline__ uint32_t run_chunk(uint32_t end, uint32_t chunk, uint
 //   Packed rows see half of their own run on average: their work is counted so, and ranges that a block of rows does not reach
 // end at once.  A block's last range is half empty on average; where that guess makes more items than places, the range is taken
 // that cannot: a second round on the device costs more than shorter ranges give.  (Counting a whole range lost per block
-// left a tenth of the device idle: trees of 24 nodes on sixteen slots of 1000 .. 4100 fp32 rows 129 us, 119 so; two trees on
-// 33,000 and 65,000 half rows 204 and 198.)
+// left a tenth of the device idle: trees of 24 nodes on sixteen slots of 1000 .. 4100 fp32 rows took 1.08 of the time so reached, now
+// 125 us; two trees on 33,000 and 65,000 half rows 1.03, now 204.)
 __device__ __forceinline__ Item item_of(const RunsCall& a, uint32_t item, uint32_t rows, bool causal)
 {
     const uint32_t lane = threadIdx.x & 63u;

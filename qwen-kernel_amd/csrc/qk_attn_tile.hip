@@ -22,9 +22,9 @@
 // What two halves hold is to 2^-22 exact while the lo half is normal, so everything that is split lies as high in a half's range as it may
 // (sums are fp32: 2^15 2^15 times the keys): elements down to 2^-16 of their row's largest are exact to 2^-22, smaller ones to 2^-39
 // of that; weights around 2^11, not 1, are to 2^-36 of the row's largest (half caches: the sum has the same factor).
-//   Bound by the matrix cores, fed from LDS.  Prompts of 8191 and 3001 rows, fp32, 16 heads on 2 of 256: 1.88 ms, 3 x 332 TFLOP/s
+//   Bound by the matrix cores, fed from LDS.  Prompts of 8191 and 3001 rows, fp32, 16 heads on 2 of 256: 1.95 ms, 3 x 320 TFLOP/s
 // of products where a large matrix product reaches 1091; three chunks of 777 .. 2048 rows behind up to 6000, half, 32 heads on 8 of 128:
-// 0.58 ms, 2 x 426 TFLOP/s.  A tile of 32 fp32 keys takes 2.2 to 2.8 us, 64 half keys 3.4 us.  A call of a few tiles is a
+// 0.60 ms, 2 x 418 TFLOP/s.  A tile of 32 fp32 keys takes 2.2 to 2.8 us, 64 half keys 3.4 us.  A call of a few tiles is a
 // chain of round trips: 9 us pass before the first product (lengths 2, queries 3, first tile 4).
 //   Tried and dropped: staging cut up between the products, which keeps both sides' registers live and spills (4.7 ms).
 #include "qk_attn_runs.h"

@@ -6,7 +6,8 @@
 // free page in ascending order.  What is to be copied goes into a list of (page, page, rows) in the workspace, and a
 // second launch over the whole device copies it for all layers, bound by memory: six copies of 1777 and 4001 rows, 20 fp32
 // heads of 256, K and V (1.4 GB moved), 284 us or 5.0 TB/s.  The books themselves are a chain of passes over the tables between
-// barriers: resize 2 to 5 us, fork 3.4 us for sixteen sequences; compaction of sixteen paths 5.8 us, three round trips.
+// barriers: resize 2 to 6 us on pools of up to 200 pages (another pass per 1024 pages that are passed over in the search for free
+// ones), fork 3.3 us for sixteen sequences; compaction of sixteen paths 5.7 us, three round trips.
 #include "qk_kv.h"
 
 #include <algorithm>
