@@ -471,13 +471,14 @@ int qkk_attn_prep_axes(const qkk_kv_cache *C_host, uint32_t layer, const qkk_kv_
  *                  of one node is the decode step.
  * A row that sees nothing gives zeros.  What a row does not see never enters its result, whatever the
  * cache holds there; what it sees and is not finite makes it NaN or infinite (an infinite key, too; only a
- * score of finite operands that passes fp32's range downwards is a weight of zero).  Value rows of an F32 cache may differ in size as far as fp32 reaches (below 2^-126 they
- * may count as zeros).
- * The softmax's maximum and sum and all sums are fp32.  Into the products go as two halves per element: the
- * queries, for an F16 cache the weights, and for an F32 cache, where a run may have more than 16 (dh 128: 32)
- * rows x heads of one KV head, keys, values and weights too.  An element is exact to 2^-22 down to 2^-16 of the
- * largest of its row, and to 2^-39 of that below; a weight (F32: weight times value row) to 2^-22 down to
- * 2^-13 of the row's largest, and to 2^-36 of that below.  Otherwise an F32 cache's operands are exact.
+ * score of finite operands that passes fp32's range downwards is a weight of zero).  Value rows of an F32
+ * cache may differ in size as far as fp32 reaches: below 2^-126 they may count as zeros, and the largest
+ * times the keys that a row sees has to stay below 2^128.
+ * The softmax's maximum and sum and all sums are fp32.  For an F16 cache queries and weights, for an F32 cache
+ * whose runs may have more than 16 (dh 128: 32) rows x heads of one KV head queries, keys, values and weights go
+ * into the products as two halves per element: exact to 2^-22 down to 2^-16 of the largest of the row, to
+ * 2^-39 of that below; a weight (F32: weight times value row) to 2^-22 down to 2^-13 of the row's largest, to
+ * 2^-36 of that below.  In the other calls an F32 cache's operands are exact.
  * The same call gives the same bits.  Into how many ranges the keys are cut, and with it the last bits of a
  * row, depends on the lengths of all runs of the call.
  *   workspace: qkk_attn_runs_workspace_bytes() (0 for sizes that the calls refuse), 256-byte aligned, no
